@@ -322,6 +322,36 @@ int tfb_exl3_down(const void* x, const int64_t* tp, const int32_t* k2, const int
 int tfb_exl3_rot_out(const float* z, const void* svh, const void* bias, void* out, int64_t out_stride, int out_type,
                      int M, int N, void* stream);
 
+/* ---- experts on 16-bit weights (no reference counterpart: its routed experts are quantised) --------------------- */
+
+/* bf16 or fp16 weights [E, n, k] (m1: the up matrix beside the gate m0, or null) into the layout the grouped product
+ * reads: out [E, mats * (n up to 16), k up to 64] in the same type; k a multiple of 8.  tfb_unpack16 inverts it bit for
+ * bit. */
+int tfb_pack16(const void* m0, const void* m1, void* out, int experts, int n, int k, void* stream);
+int tfb_unpack16(const void* packed, void* m0, void* m1, int experts, int n, int k, void* stream);
+
+/* The grouped product over a plan (tfb_plan, tfb_select_plan, tfb_route) whose items hold at most `tile` pairs (1..256):
+ * row p of out = f(x[p / slots] times the rows of expert e(p)), or x[p] when slots is 0; rows of pairs that are not in the
+ * plan are left as they are.  epi: 0 fp32 out, 1 relu^2, 2 SwiGLU over (gate, up) clipped at limit when limit > 0, 3 the
+ * sum; 1 to 3 rounded once to the weights' type (fp16 != 0: fp16, else bf16), which x has too.  x: x_rows rows of k inputs,
+ * x_stride elements apart, 16-byte aligned.  max_items: an upper bound of the plan's items.  A pair's bits depend on its own
+ * row alone. */
+int tfb_experts16(int epi, int fp16, const void* x, int64_t x_stride, int64_t x_rows, int slots, const void* w, int k,
+                  int n, const int32_t* items, const int32_t* counts, const int32_t* members, void* out, float limit,
+                  int64_t max_items, int tile, void* stream);
+
+/* ---- low-rank adapters (no reference counterpart) ------------------------------------------------------------------ */
+
+/* out[m] = base[m] + scale[i] * B[i] (A[i] x[m]) with i = ids[m], the base alone where i is outside 0..count-1.  x
+ * [rows, k], a [count, rank, k], b [count, n, rank] in bf16 or fp16 (fp16 != 0); k and rank multiples of 8, rank at most
+ * 128, zeros behind an adapter's own rank.  base and out: fp32 (0), bf16 (1) or fp16 (2) rows *_stride elements apart; out
+ * may be base.  items, counts, members, max_items: tfb_plan's tables of the ids with items of at most 64 rows, or nulls:
+ * every row on its own (for few rows).  A row's bits depend on its own row alone. */
+int tfb_adapters(int fp16, const void* x, int64_t x_stride, const void* a, const void* b, const float* scale, int rank,
+                 int k, int n, const int32_t* ids, int rows, int count, const int32_t* items, const int32_t* counts,
+                 const int32_t* members, int64_t max_items, const void* base, int base_type, int64_t base_stride,
+                 void* out, int out_type, int64_t out_stride, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -15,6 +15,7 @@ from dataclasses import dataclass, field
 import torch
 
 from .. import _lib
+from .. import adapters as low_rank
 from . import experts as routed
 
 CODEBOOK_IDS = {"3inst": routed.CB_3INST, "mcg": routed.CB_MCG, "mul1": routed.CB_MUL1}
@@ -105,9 +106,11 @@ class Exl3Linear:
         return {**st, **rows}
 
     def __call__(self, x: torch.Tensor, out: torch.Tensor | None = None, out_dtype: torch.dtype | None = None,
-                 xh: torch.Tensor | None = None, z: torch.Tensor | None = None) -> torch.Tensor:
+                 xh: torch.Tensor | None = None, z: torch.Tensor | None = None,
+                 adapters: low_rank.Adapters | None = None, plan: low_rank.Plan | None = None) -> torch.Tensor:
         """y [M, N] = x [M, K] @ W + bias for M = 1 .. MAX_ROWS; scratch ``xh`` fp16 [M, K] and ``z`` fp32 [M, N] are
-        allocated when not given.  Every 16 rows decode the trellis once (the decode form of the experts)."""
+        allocated when not given.  Every 16 rows decode the trellis once (the decode form of the experts).  ``adapters`` with
+        their ``plan`` (``adapters.route``): each row's low-rank adapter is added to the fp32 product before its rounding."""
 
         if not x.is_cuda or x.dim() != 2 or x.shape[1] != self.k or not 1 <= x.shape[0] <= MAX_ROWS:
             raise ValueError(f"x must be CUDA [1..{MAX_ROWS}, {self.k}], got {tuple(x.shape)}")
@@ -115,6 +118,12 @@ class Exl3Linear:
             raise ValueError("x must be bf16 or fp16")
         x = x.contiguous()
         m, dev = x.shape[0], x.device
+        if adapters is not None:
+            if adapters.n != self.n or adapters.k != self.k:
+                raise ValueError(f"adapters of [{adapters.n}, {adapters.k}] beside a projection of [{self.n}, {self.k}]")
+            if plan is None:
+                raise ValueError("adapters= takes the plan= of the rows' ids (adapters.Plan, adapters.route)")
+            low_rank.check(x, adapters, plan)
         t = self._tables(m)
         if xh is None:
             xh = torch.empty((m, self.k), dtype=torch.float16, device=dev)
@@ -133,6 +142,10 @@ class Exl3Linear:
         if self.bias is not None:
             y += self.bias.float()
         want = out_dtype or (out.dtype if out is not None else x.dtype)
+        if adapters is not None:
+            if out is None and want in low_rank.ROW_TYPES:
+                return low_rank.add(x, adapters, plan, y, dtype=want)
+            low_rank.add(x, adapters, plan, y, y)
         if out is None:
             return y.to(want)
         out.copy_(y)

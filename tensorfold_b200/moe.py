@@ -14,10 +14,17 @@ import torch
 
 from . import _lib
 from . import experts as grouped
+from . import experts16
 
 
 def _stream(t: torch.Tensor) -> int:
     return _lib.stream(t.device)
+
+
+def _ops(ex):
+    """The operators of a layer's kind of experts: affine 4-bit (``experts``) or 16-bit (``experts16``)."""
+
+    return experts16 if isinstance(ex, experts16.Experts16) else grouped
 
 
 def router(x: torch.Tensor, rows: torch.Tensor, out: torch.Tensor | None = None, *, prompt: bool = False) -> torch.Tensor:
@@ -44,20 +51,25 @@ def router(x: torch.Tensor, rows: torch.Tensor, out: torch.Tensor | None = None,
 
 
 class MoEBuffers:
-    """Static scratch for up to ``rows`` rows (CUDA-graph safe); ``prefill`` picks the experts' prefill arithmetic."""
+    """Static scratch for up to ``rows`` rows (CUDA-graph safe); ``prefill`` picks the experts' prefill arithmetic.
+    ``dtype``: the weights' type of 16-bit experts, which have one arithmetic; ``prefill`` then picks the router's form
+    and, for bf16, rows of the down projection that are rounded before the sum over the slots."""
 
     def __init__(self, rows: int, cfg, device: torch.device | str, *, prefill: bool = False,
-                 shared: bool = True) -> None:
+                 shared: bool = True, dtype: torch.dtype | None = None) -> None:
         extra = 1 if shared else 0
         slots = cfg.num_experts_per_tok + extra
-        self.rows, self.slots, self.shared = rows, slots, shared
+        self.rows, self.slots, self.shared, self.prefill = rows, slots, shared, prefill
         self.logits = torch.empty((rows, cfg.num_experts + extra), dtype=torch.float32, device=device)
         self.pick = torch.empty((rows, slots), dtype=torch.int32, device=device)
         self.wts = torch.empty((rows, slots), dtype=torch.float32, device=device)
-        self.plan = grouped.Plan(rows, slots, cfg.num_experts + extra, device, prefill=prefill)
-        self.act = torch.empty((rows, slots, cfg.moe_intermediate_size), dtype=torch.bfloat16, device=device)
-        self.y = torch.empty((rows, slots, cfg.hidden_size), dtype=torch.bfloat16 if prefill else torch.float32,
-                             device=device)
+        if dtype is None:
+            self.plan = grouped.Plan(rows, slots, cfg.num_experts + extra, device, prefill=prefill)
+        else:
+            self.plan = experts16.Plan(rows, slots, cfg.num_experts + extra, device)
+        self.act = torch.empty((rows, slots, cfg.moe_intermediate_size), dtype=dtype or torch.bfloat16, device=device)
+        self.y = torch.empty((rows, slots, cfg.hidden_size), device=device,
+                             dtype=torch.bfloat16 if prefill and dtype != torch.float16 else torch.float32)
         # arrival counters of the kernels that finish their work in whichever block comes last (zero between calls):
         # the one-launch routing (one a group of eight rows, plus one) and the combine folded into the down projection
         self.arrive_route = torch.zeros((2 + rows // 8,), dtype=torch.int32, device=device)
@@ -174,7 +186,8 @@ def _route_any(x: torch.Tensor, router_rows: torch.Tensor, buf: MoEBuffers, top_
             and buf.plan.experts == router_rows.shape[0]:
         route(x, router_rows, buf, top_k, experts)
         return 1
-    router(x, router_rows, buf.logits[:rows], prompt=buf.plan.prefill)
+    prompt = buf.prefill if isinstance(buf.plan, experts16.Plan) else buf.plan.prefill
+    router(x, router_rows, buf.logits[:rows], prompt=prompt)
     select(buf.logits[:rows], buf, top_k, experts, grouped.prompt_tile(rows * buf.slots, buf.plan.experts))
     return 2 if rows <= fused_select_rows() else 3
 
@@ -183,10 +196,10 @@ def moe(x: torch.Tensor, router_rows: torch.Tensor, ex: grouped.Experts, buf: Mo
         experts: int) -> MoEBuffers:
     """Route x [R, D] and run its experts into buf.y [R, slots, D] (bf16 in prefill)."""
 
-    rows = x.shape[0]
+    rows, ops = x.shape[0], _ops(ex)
     _route_any(x, router_rows, buf, top_k, experts)
-    grouped.gate_up(x, ex, buf.plan, buf.act.view(-1, ex.width), rows)
-    grouped.down(buf.act.view(-1, ex.width), ex, buf.plan, buf.y.view(-1, ex.dims), rows)
+    ops.gate_up(x, ex, buf.plan, buf.act.view(-1, ex.width), rows)
+    ops.down(buf.act.view(-1, ex.width), ex, buf.plan, buf.y.view(-1, ex.dims), rows)
     return buf
 
 
@@ -196,10 +209,11 @@ def layer(x: torch.Tensor, m: "Routed", buf: MoEBuffers, out: torch.Tensor) -> i
     five for a decode batch, six for a prompt.  buf.y still holds every slot's row.  Returns the launches made."""
 
     rows, ex = x.shape[0], m.experts
+    ops = _ops(ex)
     launches = _route_any(x, m.router, buf, m.top_k, m.count)
-    grouped.gate_up(x, ex, buf.plan, buf.act.view(-1, ex.width), rows)
-    if buf.plan.prefill or buf.plan.hot or rows > FUSED_COMBINE_ROWS:
-        grouped.down(buf.act.view(-1, ex.width), ex, buf.plan, buf.y.view(-1, ex.dims), rows)
+    ops.gate_up(x, ex, buf.plan, buf.act.view(-1, ex.width), rows)
+    if buf.plan.prefill or buf.plan.hot or rows > FUSED_COMBINE_ROWS or ops is experts16:
+        ops.down(buf.act.view(-1, ex.width), ex, buf.plan, buf.y.view(-1, ex.dims), rows)
         combine(buf.y[:rows], buf.wts[:rows], out)
         return launches + 3
     grouped.down_combine(buf.act.view(-1, ex.width), ex, buf.plan, buf.y.view(-1, ex.dims), rows, buf.wts, out,
@@ -249,7 +263,7 @@ class Routed:
     """A layer's router rows ([E + 1, D] bf16 with the shared expert's gate row last, or [E, D]) and its experts."""
 
     router: torch.Tensor
-    experts: grouped.Experts
+    experts: grouped.Experts | experts16.Experts16
     top_k: int
     shared: bool = True
 
@@ -264,6 +278,10 @@ class _Shape:
         self.moe_intermediate_size, self.hidden_size = m.experts.width, m.experts.dims
 
 
+def _weights_type(ex) -> torch.dtype | None:
+    return ex.dtype if isinstance(ex, experts16.Experts16) else None
+
+
 _scratch: dict[tuple, MoEBuffers] = {}
 
 
@@ -272,12 +290,63 @@ def run(x: torch.Tensor, m: Routed, *, prefill: bool = False) -> torch.Tensor:
 
     rows = x.shape[0]
     size = 1 << max(4, (rows - 1).bit_length())                 # scratch per power of two, reused by every layer
-    key = (size, m.count, m.top_k, m.experts.width, m.experts.dims, prefill, m.shared, x.device)
+    dtype = _weights_type(m.experts)
+    key = (size, m.count, m.top_k, m.experts.width, m.experts.dims, prefill, m.shared, x.device, dtype)
     buf = _scratch.get(key)
     if buf is None:
-        buf = _scratch[key] = MoEBuffers(size, _Shape(m), x.device, prefill=prefill, shared=m.shared)
+        buf = _scratch[key] = MoEBuffers(size, _Shape(m), x.device, prefill=prefill, shared=m.shared, dtype=dtype)
     out = torch.empty((rows, m.experts.dims), dtype=torch.bfloat16, device=x.device)
     layer(x.contiguous(), m, buf, out)
+    return out
+
+
+class _Picked:
+    def __init__(self, ex, slots: int) -> None:
+        self.num_experts_per_tok, self.num_experts = slots, ex.count
+        self.moe_intermediate_size, self.hidden_size = ex.width, ex.dims
+
+
+def buffers(ex, rows: int, slots: int, *, prefill: bool = False) -> MoEBuffers:
+    """``MoEBuffers`` for ``picked``: up to ``rows`` rows of ``slots`` experts each."""
+
+    return MoEBuffers(rows, _Picked(ex, slots), ex.up.device, prefill=prefill, shared=False, dtype=_weights_type(ex))
+
+
+def picked(x: torch.Tensor, ex, picks: torch.Tensor, wts: torch.Tensor, *, buf: MoEBuffers | None = None,
+           out: torch.Tensor | None = None) -> torch.Tensor:
+    """The experts and weights a caller's own routing picked: x [R, D], picks [R, slots] int32, wts [R, slots] fp32 ->
+    [R, D] = the sum over the slots of wts * expert(x), for either kind of experts.  A slot whose pick is outside 0..E-1
+    takes no part, whatever its weight; a row without any comes out as zeros.  The result is bf16, or fp32 when ``out`` is
+    (always, for fp16 experts).  ``buf`` (``buffers``) is scratch a program keeps; without it the call allocates its own."""
+
+    rows, slots = picks.shape if picks.dim() == 2 else (-1, -1)
+    if picks.dim() != 2 or x.dim() != 2 or x.shape[0] != rows or x.shape[1] != ex.dims or slots < 1:
+        raise ValueError(f"picked: x [R, {ex.dims}] and picks [R, slots], not {tuple(x.shape)} and {tuple(picks.shape)}")
+    if not x.is_cuda or picks.device != x.device or wts.device != x.device:
+        raise ValueError("picked: x, picks and wts must be on one CUDA device (this library has no CPU path)")
+    if wts.dtype != torch.float32 or wts.shape != picks.shape or not wts.is_contiguous():
+        raise ValueError(f"picked: wts must be contiguous fp32 {tuple(picks.shape)}")
+    if buf is None:
+        buf = buffers(ex, max(rows, 1), slots, prefill=False)
+    if buf.slots != slots or rows > buf.rows or buf.plan.experts != ex.count or buf.act.shape[2] != ex.width \
+            or buf.y.shape[2] != ex.dims:
+        raise ValueError(f"picked: {rows} rows of {slots} do not fit buffers of {buf.rows} x {buf.slots}")
+    half = _weights_type(ex) == torch.float16
+    if out is None:
+        out = torch.empty((rows, ex.dims), dtype=torch.float32 if half else torch.bfloat16, device=x.device)
+    elif tuple(out.shape) != (rows, ex.dims) or not out.is_contiguous() or out.device != x.device \
+            or out.dtype not in ((torch.float32,) if half else (torch.bfloat16, torch.float32)):
+        raise ValueError(f"picked: out must be contiguous [{rows}, {ex.dims}] bf16 or fp32 (fp32 for fp16 experts)")
+    if rows == 0:
+        return out
+    ops = _ops(ex)
+    grouped.route(picks, buf.plan, grouped.prompt_tile(rows * slots, ex.count))
+    ops.gate_up(x, ex, buf.plan, buf.act.view(-1, ex.width), rows)
+    ops.down(buf.act.view(-1, ex.width), ex, buf.plan, buf.y.view(-1, ex.dims), rows)
+    with _lib.on(x.device):
+        _lib.call("tfb_combine_window", buf.y.data_ptr(), 1 if buf.y.dtype == torch.bfloat16 else 0, wts.data_ptr(),
+                  picks.data_ptr(), 0, ex.count, out.data_ptr(), 1 if out.dtype == torch.float32 else 0, rows, slots, ex.dims,
+                  _stream(x))
     return out
 
 
@@ -293,7 +362,7 @@ class Runner:
         device = torch.device(device if device is not None else m.router.device)
         self.layer, self.rows, self.prefill = m, rows, prefill
         self.x = torch.zeros((rows, m.experts.dims), dtype=torch.bfloat16, device=device)
-        self.buf = MoEBuffers(rows, _Shape(m), device, prefill=prefill, shared=m.shared)
+        self.buf = MoEBuffers(rows, _Shape(m), device, prefill=prefill, shared=m.shared, dtype=_weights_type(m.experts))
         self.out = torch.zeros((rows, m.experts.dims), dtype=torch.bfloat16, device=device)
         self._stream = torch.cuda.Stream(device)
         with torch.cuda.device(device):

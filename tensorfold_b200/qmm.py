@@ -19,6 +19,7 @@ from types import SimpleNamespace
 import torch
 
 from . import _lib
+from . import adapters as low_rank
 from . import experts as grouped
 
 _PLANS: dict = {}
@@ -134,18 +135,38 @@ def _run(x: torch.Tensor, q: Q4, f32: bool, out: torch.Tensor | None, prefill: b
     return out
 
 
+def _adapted(x: torch.Tensor, q: Q4, f32: bool, out: torch.Tensor | None, prefill: bool, adapters, plan) -> torch.Tensor:
+    """The product left in fp32, each row's adapter on top of it, one rounding."""
+
+    if adapters.n != q.n or adapters.k != q.k:
+        raise ValueError(f"adapters of [{adapters.n}, {adapters.k}] beside a projection of [{q.n}, {q.k}]")
+    if plan is None:
+        raise ValueError("adapters= takes the plan= of the rows' ids (adapters.Plan, adapters.route)")
+    low_rank.check(x, adapters, plan)
+    want = torch.float32 if f32 else torch.bfloat16
+    if out is not None and (out.shape != (x.shape[0], q.n) or out.dtype != want or not out.is_contiguous()):
+        raise ValueError(f"out must be contiguous ({x.shape[0]}, {q.n}) {want}")
+    return low_rank.add(x, adapters, plan, _run(x, q, True, None, prefill), out, dtype=want)
+
+
 def matmul(x: torch.Tensor, q: Q4, xs: torch.Tensor | None = None, *, sk: int | None = None, f32: bool = False,
-           out: torch.Tensor | None = None, part: torch.Tensor | None = None, reduce: bool = True) -> torch.Tensor:
+           out: torch.Tensor | None = None, part: torch.Tensor | None = None, reduce: bool = True,
+           adapters: low_rank.Adapters | None = None, plan: low_rank.Plan | None = None) -> torch.Tensor:
     """x @ q.T as (M, n) bf16, or unrounded fp32 with ``f32``: exact integer products per group, then
     ``acc = fma(xs, b, fma(p, s, acc))`` in fp32 (the decode arithmetic).  ``reduce=False`` returns the K slices apart,
     fp32 (split_k, M, n) (in ``part`` when given), for a caller that adds them in slice order inside its next kernel;
     with one slice it returns the product itself, as the reference does
-    (``src/tensorfold/cuda/kernels/qmm.py:156-177``)."""
+    (``src/tensorfold/cuda/kernels/qmm.py:156-177``).  ``adapters`` with their ``plan``: each row's low-rank adapter is added
+    to the fp32 product before its one rounding."""
 
     slices = split_k(q.n, q.k, q.gs)
     if sk is not None and sk != slices:
         raise ValueError("matmul: the K slicing is the shape's (split_k), it cannot be chosen per call")
     x = _check(x, q, "matmul")
+    if adapters is not None:
+        if not reduce:
+            raise ValueError("matmul: adapters are added to the whole product, not to its slices (reduce=False)")
+        return _adapted(x, q, f32, out, False, adapters, plan)
     if reduce or slices == 1:
         return _run(x, q, f32, out, False)
     return _slices(x, q, slices, part)
@@ -175,9 +196,11 @@ def _slices(x: torch.Tensor, q: Q4, slices: int, part: torch.Tensor | None) -> t
     return view
 
 
-def prefill_matmul(x: torch.Tensor, q: Q4, *, f32: bool = False, tile: int = 0,
-                   out: torch.Tensor | None = None) -> torch.Tensor:
+def prefill_matmul(x: torch.Tensor, q: Q4, *, f32: bool = False, tile: int = 0, out: torch.Tensor | None = None,
+                   adapters: low_rank.Adapters | None = None, plan: low_rank.Plan | None = None) -> torch.Tensor:
     """Prefill: weights rounded once to bf16, one fp32 chain over K (tcgen05); any chunking gives the same bits, not
-    ``matmul``'s."""
+    ``matmul``'s.  ``adapters`` and ``plan`` as in ``matmul``."""
 
+    if adapters is not None:
+        return _adapted(_check(x, q, "prefill_matmul"), q, f32, out, True, adapters, plan)
     return _run(_check(x, q, "prefill_matmul"), q, f32, out, True)
