@@ -65,9 +65,6 @@ __device__ __forceinline__ void ad_store(void* p, int type, int64_t i, float v) 
   else static_cast<uint16_t*>(p)[i] = type == AD_BF16 ? to16<false>(v) : to16<true>(v);
 }
 
-__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;\n" ::: "memory"); }
-__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;\n" ::: "memory"); }
-
 // the float4 at `p` of this CTA's shared memory, in the same place of CTA `rank` of the cluster
 __device__ __forceinline__ float4 ld_cluster4(const float* p, int rank) {
   uint32_t at;

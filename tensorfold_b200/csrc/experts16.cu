@@ -11,6 +11,9 @@
 #include "api.h"
 #include "common.cuh"
 
+#include <cuda.h>
+#include <cudaTypedefs.h>
+
 namespace tfb {
 
 // ---- packed weights --------------------------------------------------------------------------------------------------
@@ -67,18 +70,40 @@ unpack16_kernel(const uint4* packed, uint8_t* m0, uint8_t* m1, int mats, int n, 
 }
 
 // ---- the grouped product ---------------------------------------------------------------------------------------------
+// Persistent: the CTAs (CG = 1), or pairs of CTAs whose tensor cores work as one (CG = 2), walk units = (item, CG * RU rows
+// of its expert's weights).  A CTA's roles run apart, each through all of its units, so that the copies of the next unit
+// travel while the last one is finished:
+//   warp 5     the weights' bulk copies: RU rows;  warps 6-9 the pairs' input rows by TMA gathers (four rows an instruction,
+//              zeros behind the last input), of a pair of CTAs each one half; both into a ring of stages of 128 / RU blocks
+//              of 64 inputs, 16 KB of weights each;
+//   warp 4     one lane (of a pair's first CTA, on whose barriers both CTAs' copies count) issues tcgen05.mma (M = 128 CG, N =
+//              pairs) into one of two accumulators in tensor memory;
+//   warps 0-3  read the other accumulator, apply the activation and store the pairs' rows: through shared memory, where a
+//              lane's one column of many pairs becomes 16 bytes of a pair's row.  (Stored from the registers, 2 bytes a
+//              lane, a unit of 256 pairs took 14 us to finish where its products take 3 to 9.)
 constexpr int G16_MAXP = 256;                      // pairs an item may hold (MMA N)
-constexpr int G16_THREADS = 192;                   // warps 0-3 gather and finish, 4 issues the MMAs, 5 copies the weights
+constexpr int G16_B_WARPS = 4;
+constexpr int G16_MMA_WARP = 4, G16_A_WARP = 5, G16_B_WARP = 6;
+constexpr int G16_THREADS = (G16_B_WARP + G16_B_WARPS) * 32;
 
-template <int MAXP>
-struct G16Smem {
-  static constexpr int A_BYTES = W16_ROWS * 128, B_BYTES = MAXP * 128;
-  static constexpr int STAGES = 4;
-  static constexpr int TABLE_OFFSET = STAGES * (A_BYTES + B_BYTES);        // int pair[MAXP]
-  static constexpr int BAR_OFFSET = TABLE_OFFSET + MAXP * 4;
-  static constexpr int TMEM_OFFSET = BAR_OFFSET + (2 * STAGES + 1) * 8;
+template <int CG, int MAXP, int RU>
+struct G16Shape {
+  static constexpr int KPS = W16_ROWS / RU;                                // blocks of 64 inputs a stage
+  static constexpr int A_BYTES = W16_ROWS * 128, B_BLOCK = MAXP / CG * 128, B_BYTES = KPS * B_BLOCK;
+  static constexpr int STAGE = A_BYTES + B_BYTES;
+  static constexpr int STAGES = (214 * 1024 / STAGE) < 10 ? (214 * 1024 / STAGE) : 10;
+  static constexpr int TABLE_OFFSET = STAGES * STAGE;                      // int pair[2][MAXP]
+  static constexpr int TURN_OFFSET = TABLE_OFFSET + 2 * MAXP * 4;          // the finishing warps' rows: 2 KB each
+  static constexpr int BAR_OFFSET = TURN_OFFSET + 4 * 2048;
+  static constexpr int TMEM_OFFSET = BAR_OFFSET + (2 * STAGES + 4) * 8;
   static constexpr int TOTAL = TMEM_OFFSET + 16 + 1024;                    // + slack to align the tiles to 1024 bytes
+  static constexpr int ACC_COLS = MAXP;                                    // tensor memory: two accumulators
+  static constexpr int STEP = 16 * CG;                                     // N is a multiple of it
+  static constexpr int LANES = MAXP / CG / 4 / G16_B_WARPS;                // lanes of a gathering warp with a group of rows
   static_assert(TOTAL <= 227 * 1024, "one CTA's shared memory");
+  static_assert(ACC_COLS >= 32 && 2 * ACC_COLS <= 512 && LANES >= 1 && LANES <= 32, "tensor memory; the gathers");
+  static_assert((KPS - 1) * RU * 128 + A_BYTES <= STAGE, "an operand of 128 rows of which RU are this unit's stays in its stage");
+  static_assert(CG == 1 || RU == W16_ROWS, "a pair of CTAs takes whole tiles");
 };
 
 template <bool F16>
@@ -97,198 +122,471 @@ __device__ __forceinline__ float swiglu32(float g, float u, float limit) {
   return __fdividef(g, 1.f + __expf(-g)) * u;
 }
 
+template <int CG>
 __device__ __forceinline__ void umma_ss(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accum) {
+  if constexpr (CG == 1)
+    asm volatile(
+        "{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\n"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d_tmem),
+        "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accum)
+        : "memory");
+  else
+    asm volatile(
+        "{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\n"
+        "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d_tmem),
+        "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accum)
+        : "memory");
+}
+
+// kind::f16, D fp32, both operands K-major, bf16 or fp16, M = 128 CG, N = n
+template <int CG, bool F16>
+__device__ __forceinline__ uint32_t g16_idesc(int n) {
+  const uint32_t type = F16 ? 0u : 1u;
+  return (1u << 4) | (type << 7) | (type << 10) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(CG * W16_ROWS >> 4) << 24);
+}
+
+// The MMAs so far have retired: one arrival on the barrier, of a pair of CTAs on both CTAs' barriers in that place.
+template <int CG>
+__device__ __forceinline__ void g16_commit(uint64_t* bar) {
+  if constexpr (CG == 1)
+    umma_commit(bar);
+  else
+    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;\n" ::"r"(
+                     smem_addr(bar)),
+                 "h"((uint16_t)3)
+                 : "memory");
+}
+
+__device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&r)[32]) {
   asm volatile(
-      "{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\n"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d_tmem),
-      "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accum)
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
+      "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];\n"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+        "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(taddr));
+}
+
+template <int CG>
+__device__ __forceinline__ void g16_alloc(uint32_t* dst_smem, uint32_t ncols) {
+  if constexpr (CG == 1) {
+    tmem_alloc(dst_smem, ncols);
+  } else {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(smem_addr(dst_smem)), "r"(ncols)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;\n" ::: "memory");
+  }
+}
+template <int CG>
+__device__ __forceinline__ void g16_dealloc(uint32_t taddr, uint32_t ncols) {
+  if constexpr (CG == 1) tmem_dealloc(taddr, ncols);
+  else asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;\n" ::"r"(taddr), "r"(ncols) : "memory");
+}
+
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %cluster_ctarank;\n" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;\n" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;\n" ::: "memory"); }
+
+// The first CTA's barrier (or other shared memory) in the place of this CTA's, as a shared::cluster address.
+__device__ __forceinline__ uint32_t leader_addr(const void* p) {
+  uint32_t at;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, 0;\n" : "=r"(at) : "r"(smem_addr(p)));
+  return at;
+}
+__device__ __forceinline__ void mbar_arrive_leader(uint64_t* bar) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];\n" ::"r"(leader_addr(bar)) : "memory");
+}
+
+// mbar_wait for a barrier on which the other CTA of the pair arrives too.  (Once a unit: with this scope a wait costs half a
+// microsecond, which at every stage was most of the kernel's time.)
+__device__ __forceinline__ bool mbar_wait_cluster(uint64_t* bar, uint32_t parity) {
+  if (!mbar_wait(bar, parity)) return false;
+  asm volatile("fence.acq_rel.cluster;\n" ::: "memory");
+  return true;
+}
+
+// Four rows' 64 inputs from column `col` on into 512 bytes of a swizzled operand tile; zeros behind the map's columns.  `bar`:
+// a shared::cluster address; of a pair of CTAs both count on the first one's barrier.
+template <int CG>
+__device__ __forceinline__ void tma_gather4(void* dst, const CUtensorMap* map, int col, int4 r, uint32_t bar) {
+  if constexpr (CG == 1)
+    asm volatile(
+        "cp.async.bulk.tensor.2d.shared::cta.global.tile::gather4.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5, "
+        "%6}], [%7];\n" ::"r"(smem_addr(dst)),
+        "l"(map), "r"(col), "r"(r.x), "r"(r.y), "r"(r.z), "r"(r.w), "r"(bar)
+        : "memory");
+  else
+    asm volatile(
+        "cp.async.bulk.tensor.2d.shared::cluster.global.tile::gather4.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, "
+        "{%2, %3, %4, %5, %6}], [%7];\n" ::"r"(smem_addr(dst)),
+        "l"(map), "r"(col), "r"(r.x), "r"(r.y), "r"(r.z), "r"(r.w), "r"(bar)
+        : "memory");
+}
+
+// A tile of whole rows of the packed weights, as they are, for one CTA of a pair.
+__device__ __forceinline__ void tma_rows_pair(void* dst, const CUtensorMap* map, int row, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, {%2, %3}], "
+      "[%4];\n" ::"r"(smem_addr(dst)),
+      "l"(map), "r"(0), "r"(row), "r"(bar)
       : "memory");
 }
 
-// kind::f16, D fp32, both operands K-major, bf16 or fp16, M = 128, N = n
-template <bool F16>
-__device__ __forceinline__ uint32_t g16_idesc(int n) {
-  const uint32_t type = F16 ? 0u : 1u;
-  return (1u << 4) | (type << 7) | (type << 10) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(W16_ROWS >> 4) << 24);
-}
+struct RingAt {                                     // a walk around the ring of stages
+  int s = 0;
+  uint32_t ph = 0;
+  int steps = 0;
+  __device__ __forceinline__ void next(int stages) {
+    ++steps;
+    if (++s == stages) {
+      s = 0;
+      ph ^= 1;
+    }
+  }
+  // after a wait that ran out: gives the copies in flight of the last round a while to land (`here`: they count on this CTA's
+  // barriers)
+  __device__ __forceinline__ void drain(uint64_t* full, int stages, bool here) {
+    const uint64_t start = global_ns();
+    while (!here && global_ns() - start < 10000000ull) {
+    }
+    if (!here) return;
+    for (int i = min(steps, stages); i > 0; --i) {
+      ph ^= s == 0;
+      s = s == 0 ? stages - 1 : s - 1;
+      mbar_wait_for(full + s, ph, 10000000ull);
+    }
+  }
+};
 
-__device__ __forceinline__ void cp_async16_or_zero(void* dst, const void* src, bool have) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(smem_addr(dst)), "l"(src), "r"(have ? 16 : 0)
-               : "memory");
-}
-
-template <int M, int EPI, bool F16, int MAXP>
-__global__ void __launch_bounds__(G16_THREADS)
-g16_kernel(const uint16_t* __restrict__ X, int64_t x_stride, int slots, const uint8_t* __restrict__ W, int K, int N,
+// Every role reads what it needs of the plan one unit ahead: behind the last copy of a unit the chain item -> members ->
+// rows took 2 us in which the ring ran dry.
+template <int CG, int M, int EPI, bool F16, int MAXP, int RU>
+__global__ void __launch_bounds__(G16_THREADS, 1)
+g16_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ CUtensorMap wmap, int slots, const uint8_t* __restrict__ W, int K, int N,
            const int* __restrict__ items, const int* __restrict__ counts, const int* __restrict__ members,
            void* __restrict__ out, float limit) {
-  using SM = G16Smem<MAXP>;
-  constexpr int STAGES = SM::STAGES;
+  using SH = G16Shape<CG, MAXP, RU>;
+  constexpr int STAGES = SH::STAGES, KPS = SH::KPS;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint8_t* a_ring = smem;
-  uint8_t* b_ring = smem + STAGES * SM::A_BYTES;
-  int* pair = reinterpret_cast<int*>(smem + SM::TABLE_OFFSET);
-  uint64_t* full = reinterpret_cast<uint64_t*>(smem + SM::BAR_OFFSET);     // [STAGES] weights and inputs landed
+  int* table = reinterpret_cast<int*>(smem + SH::TABLE_OFFSET);
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + SH::BAR_OFFSET);     // [STAGES] weights and inputs landed
   uint64_t* empty = full + STAGES;                                         // [STAGES] the MMAs that read them retired
-  uint64_t* done = empty + STAGES;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + SM::TMEM_OFFSET);
+  uint64_t* acc_full = empty + STAGES;                                     // [2] a unit's sums are complete
+  uint64_t* acc_free = acc_full + 2;                                       // [2] and have been read
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + SH::TMEM_OFFSET);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int rows = w16_rows(M, N), KB = w16_kblocks(K), nct = (rows + W16_ROWS - 1) / W16_ROWS;
-  const int it = blockIdx.x / nct, ct = blockIdx.x - it * nct;
+  const int cta = CG == 1 ? 0 : (int)cluster_rank();                       // of the pair; 0 issues the MMAs
+  const int rows = w16_rows(M, N), KB = w16_kblocks(K), nct = (rows + CG * RU - 1) / (CG * RU);
+  const int fills = (KB + KPS - 1) / KPS;                                  // stages a unit takes
+  const int u0 = blockIdx.x / CG, du = gridDim.x / CG;
 
   if (tid == 0) {
     for (int s = 0; s < STAGES; ++s) {
-      mbar_init(full + s, 1 + 128);
+      // every warp that waits for `empty` arrives here or has copies that do: one that had no part in a stage could fall a
+      // round behind and mistake the barrier's phase
+      mbar_init(full + s, 1 + G16_B_WARPS);
       mbar_init(empty + s, 1);
     }
-    mbar_init(done, 1);
+    for (int s = 0; s < 2; ++s) {
+      mbar_init(acc_full + s, 1);
+      mbar_init(acc_free + s, 4 * CG);
+    }
     mbar_fence_init();
     fence_async_smem();
   }
+  if (warp == G16_MMA_WARP) g16_alloc<CG>(tmem_slot, 2 * SH::ACC_COLS);
   pdl_wait();
-  after_wait(X, items, counts, members);
-  const bool live = it < ld_dep(counts);                                   // uniform over the CTA
-  if (live && warp == 4) tmem_alloc(tmem_slot, MAXP);
-  int e = 0, cnt = 0;
-  if (live) {
-    e = ld_dep(items + 3 * it);
-    const int first = ld_dep(items + 3 * it + 1);
-    cnt = min(ld_dep(items + 3 * it + 2), MAXP);
-    for (int i = tid; i < cnt; i += G16_THREADS) pair[i] = ld_dep(members + first + i);
-  }
+  after_wait(items, counts, members);
   tc_fence_before();
   __syncthreads();
+  if constexpr (CG == 2) {
+    cluster_arrive();
+    cluster_wait();
+  }
   tc_fence_after();
-  if (!live) return;
   const uint32_t tmem_base = *tmem_slot;
-  const int nmma = (cnt + 15) & ~15;
-  const int rt = min(W16_ROWS, rows - ct * W16_ROWS);
+  const int units = ld_dep(counts) * nct;
   bool ok = true;
+  auto item = [&](int u) { return min(u, units - 1) / nct; };              // of the next unit, or any where there is none
 
-  if (warp == 5) {
-    const uint8_t* src = W + ((size_t)e * rows + (size_t)ct * W16_ROWS) * KB * 128;
-    int g = 0;
-    for (; g < KB; ++g) {
-      const int s = g % STAGES;
-      if (g >= STAGES) ok = mbar_wait_warp(empty + s, (g / STAGES - 1) & 1);
-      if (!ok) break;
-      if (lane == 0) {
-        mbar_expect_tx(full + s, (uint32_t)rt * 128);
-        bulk_g2s(a_ring + s * SM::A_BYTES, src + (size_t)g * rt * 128, rt * 128, full + s);
+  if (units == 0) {
+  } else if (warp == G16_A_WARP) {
+    if (lane == 0) {
+      RingAt at;
+      int e = ld_dep(items + 3 * item(u0));
+      for (int u = u0; u < units && ok; u += du) {
+        const int r0 = ((u - u / nct * nct) * CG + cta) * RU;
+        const int t0 = CG == 2 && r0 >= rows ? 0 : r0 / W16_ROWS * W16_ROWS;   // a second CTA without rows multiplies any
+        const int rt = min(W16_ROWS, rows - t0), ru = min(RU, rows - r0);
+        const uint8_t* src = W + ((size_t)e * rows + t0) * KB * 128 + (r0 - t0) * 128;
+        const int row = (e * rows + t0) * KB;
+        e = ld_dep(items + 3 * item(u + du));
+        for (int f = 0; f < fills; ++f) {
+          ok = mbar_wait(empty + at.s, at.ph ^ 1);                         // the ring's first round finds every stage free
+          if (!ok) break;
+          uint8_t* dst = smem + at.s * SH::STAGE;
+          if constexpr (CG == 1) {
+            const int nkb = min(KPS, KB - f * KPS);
+            mbar_expect_tx(full + at.s, (uint32_t)(nkb * ru) * 128);
+            for (int b = 0; b < nkb; ++b)
+              bulk_g2s(dst + b * (RU * 128), src + (size_t)(f * KPS + b) * rt * 128, ru * 128, full + at.s);
+          } else {                                                         // 128 rows: behind a shorter tile's, the next block's
+            if (cta == 0) mbar_expect_tx(full + at.s, 2 * SH::A_BYTES);
+            tma_rows_pair(dst, &wmap, row + f * rt, leader_addr(full + at.s));
+          }
+          at.next(STAGES);
+        }
+      }
+      if (!ok) at.drain(full, STAGES, cta == 0);
+    }
+    __syncwarp();
+  } else if (warp >= G16_B_WARP) {
+    // Lane l of warp w takes group l * B_WARPS + w of four rows.  (One lane's gathers follow one another every 130 ns, those
+    // of a warp's lanes every 41.)
+    const int g = lane * G16_B_WARPS + warp - G16_B_WARP;
+    RingAt at;
+    int4 next;
+    int next_cnt;
+    auto fetch = [&](int u) {
+      const int it = item(u);
+      const int first = ld_dep(items + 3 * it + 1);
+      next_cnt = min(ld_dep(items + 3 * it + 2), MAXP);
+      const int half = (next_cnt + SH::STEP - 1) / SH::STEP * SH::STEP / CG;   // pairs of this CTA
+      const int p = cta * half + 4 * g;                                    // rows past the last pair repeat it: never stored
+      if (lane < SH::LANES) {
+        next.x = ld_dep(members + first + min(p, next_cnt - 1));
+        next.y = ld_dep(members + first + min(p + 1, next_cnt - 1));
+        next.z = ld_dep(members + first + min(p + 2, next_cnt - 1));
+        next.w = ld_dep(members + first + min(p + 3, next_cnt - 1));
+      }
+    };
+    fetch(u0);
+    for (int u = u0; u < units && ok; u += du) {
+      int4 r = next;
+      if (slots) r = make_int4(r.x / slots, r.y / slots, r.z / slots, r.w / slots);
+      const int groups = (next_cnt + SH::STEP - 1) / SH::STEP * SH::STEP / CG / 4;     // of this CTA: a multiple of B_WARPS
+      fetch(u + du);
+      for (int f = 0; f < fills; ++f) {
+        ok = mbar_wait_warp(empty + at.s, at.ph ^ 1);
+        if (!ok) break;
+        const int nkb = min(KPS, KB - f * KPS);
+        uint8_t* dst = smem + at.s * SH::STAGE + SH::A_BYTES + g * 512;
+        if (lane == 0 && cta == 0) mbar_expect_tx(full + at.s, (uint32_t)(CG * nkb * (groups / G16_B_WARPS)) * 512);
+        __syncwarp();
+        const uint32_t bar = CG == 1 ? smem_addr(full + at.s) : leader_addr(full + at.s);
+        if (lane < SH::LANES && g < groups)
+          for (int b = 0; b < nkb; ++b) tma_gather4<CG>(dst + b * SH::B_BLOCK, &xmap, (f * KPS + b) * W16_K, r, bar);
+        __syncwarp();
+        at.next(STAGES);
       }
     }
-    if (!ok && lane == 0)                                                  // give the copies in flight a while to land
-      for (int f = max(0, g - STAGES); f < g; ++f) mbar_wait_for(full + f % STAGES, (f / STAGES) & 1, 10000000ull);
+    if (!ok) at.drain(full, STAGES, cta == 0);
     __syncwarp();
-  } else if (warp == 4) {
-    if (lane == 0) {
-      const uint32_t idesc = g16_idesc<F16>(nmma);
-      const uint64_t a0 = umma_desc(smem_addr(a_ring)), b0 = umma_desc(smem_addr(b_ring));
-      for (int g = 0; g < KB; ++g) {
-        const int s = g % STAGES;
-        ok = mbar_wait(full + s, (g / STAGES) & 1);
+  } else if (warp == G16_MMA_WARP) {
+    if (lane == 0 && cta == 0) {
+      const uint64_t a0 = umma_desc(smem_addr(smem)), b0 = umma_desc(smem_addr(smem + SH::A_BYTES));
+      RingAt at;
+      int n = 0;                                                           // the CTA's n-th unit
+      int next_cnt = ld_dep(items + 3 * item(u0) + 2);
+      for (int u = u0; u < units && ok; u += du, ++n) {
+        const int cnt = min(next_cnt, MAXP);
+        next_cnt = ld_dep(items + 3 * item(u + du) + 2);
+        const uint32_t idesc = g16_idesc<CG, F16>((cnt + SH::STEP - 1) / SH::STEP * SH::STEP);
+        const uint32_t acc = tmem_base + (n & 1) * SH::ACC_COLS;
+        ok = CG == 1 ? mbar_wait(acc_free + (n & 1), ((n >> 1) & 1) ^ 1) : mbar_wait_cluster(acc_free + (n & 1), ((n >> 1) & 1) ^ 1);
         if (!ok) break;
         tc_fence_after();
-        const uint64_t ad = a0 + (uint32_t)(s * (SM::A_BYTES >> 4)), bd = b0 + (uint32_t)(s * (SM::B_BYTES >> 4));
+        for (int f = 0; f < fills; ++f) {
+          ok = mbar_wait(full + at.s, at.ph);
+          if (!ok) break;
+          tc_fence_after();
+          const int nkb = min(KPS, KB - f * KPS);
+          for (int b = 0; b < nkb; ++b) {
+            const uint64_t ad = a0 + (uint32_t)((at.s * SH::STAGE + b * (RU * 128)) >> 4);
+            const uint64_t bd = b0 + (uint32_t)((at.s * SH::STAGE + b * SH::B_BLOCK) >> 4);
 #pragma unroll
-        for (int ks = 0; ks < 4; ++ks) umma_ss(tmem_base, ad + 2 * ks, bd + 2 * ks, idesc, (g | ks) ? 1u : 0u);
-        umma_commit(empty + s);
+            for (int ks = 0; ks < 4; ++ks) umma_ss<CG>(acc, ad + 2 * ks, bd + 2 * ks, idesc, (f | b | ks) ? 1u : 0u);
+          }
+          g16_commit<CG>(empty + at.s);
+          at.next(STAGES);
+        }
+        if (ok) g16_commit<CG>(acc_full + (n & 1));
       }
-      if (ok) umma_commit(done);
     }
     __syncwarp();
   } else {
-    // thread -> chunk c of rows r0, r0 + 16, ...; rows past the last pair repeat it: their columns are never stored
-    const int c = tid & 7, r0 = tid >> 3;
-    const uint32_t at = (uint32_t)(r0 * 128 + ((c ^ (r0 & 7)) << 4));
-    for (int g = 0; g < KB; ++g) {
-      const int s = g % STAGES;
-      if (g >= STAGES) ok = mbar_wait_warp(empty + s, (g / STAGES - 1) & 1);
+    // ---- the finishing warps: tensor-memory lane = weight row, column = pair ----
+    const int q = warp;
+    uint8_t* turn = smem + SH::TURN_OFFSET + q * 2048;
+    int n = 0;
+    int first = ld_dep(items + 3 * item(u0) + 1), cnt = ld_dep(items + 3 * item(u0) + 2);
+    for (int u = u0; u < units && ok; u += du, ++n) {
+      const int r0 = ((u - u / nct * nct) * CG + cta) * RU, have = min(cnt, MAXP);
+      int* pair = table + (n & 1) * MAXP;
+      for (int i = tid; i < ((have + 31) & ~31); i += 128) pair[i] = i < have ? ld_dep(members + first + i) : -1;
+      first = ld_dep(items + 3 * item(u + du) + 1);
+      cnt = ld_dep(items + 3 * item(u + du) + 2);
+      asm volatile("bar.sync 1, 128;\n" ::: "memory");
+      ok = mbar_wait_warp(acc_full + (n & 1), (n >> 1) & 1);
       if (!ok) break;
-      const int k = g * W16_K + c * 8;
-      for (int r = r0, j = 0; r < nmma; r += 16, ++j) {
-        const int p = pair[min(r, cnt - 1)];
-        const uint16_t* src = X + (size_t)(slots ? p / slots : p) * x_stride;
-        cp_async16_or_zero(b_ring + s * SM::B_BYTES + at + j * (16 * 128), src + (k < K ? k : 0), k < K);
-      }
-      cp_async_commit();
-      if (g >= 1) {                                                        // the stage before this one has landed
-        cp_async_wait<1>();
-        fence_async_smem();
-        mbar_arrive(full + (g - 1) % STAGES);
-      }
-    }
-    cp_async_wait<0>();
-    fence_async_smem();
-    if (ok) mbar_arrive(full + (KB - 1) % STAGES);
-    // ---- epilogue: tensor-memory lane = weight row, column = pair ----
-    if (ok) ok = mbar_wait_warp(done, 0);
-    if (ok) {
       tc_fence_after();
-      const int q = warp;
-      const uint32_t taddr = tmem_base + ((uint32_t)(q * 32) << 16);
-      const int col = M == 1 ? ct * W16_ROWS + q * 32 + lane : ct * (W16_ROWS / 2) + q * 16 + (lane & 15);
-      for (int j0 = 0; j0 < nmma; j0 += 16) {
-        uint32_t a[16];
-        tmem_ld16(taddr + j0, a);
+      const uint32_t taddr = tmem_base + (n & 1) * SH::ACC_COLS + ((uint32_t)(q * 32) << 16);
+      constexpr int OUT = EPI == EPI_F32 ? 4 : 2;                          // bytes of a value
+      constexpr int COLS_W = M == 1 ? 32 : 16;                             // columns a warp holds
+      constexpr int TURN = EPI == EPI_F32 ? 16 : 32;                       // pairs a turn: 2 KB or 1
+      constexpr int CHUNKS = COLS_W * OUT / 16;                            // 16-byte pieces of a pair's row
+      const int c0 = r0 / M + q * COLS_W;                                  // the warp's first column
+      const bool wide = ((size_t)N * OUT) % 16 == 0 && (reinterpret_cast<uintptr_t>(out) & 15) == 0;
+      for (int j0 = 0; j0 < have && q * 32 < RU && c0 < N; j0 += TURN) {
+        uint32_t a[32];
+        if constexpr (TURN == 32) tmem_ld32(taddr + j0, a);
+        else tmem_ld16(taddr + j0, *reinterpret_cast<uint32_t(*)[16]>(a));
         tmem_ld_wait();
+        __syncwarp();                                                      // the turn before this one has been read
         if constexpr (M == 2) {
           // a column's gate and up rows sit 16 lanes apart: of two neighbouring pairs the gate lane forms the first
           // and the up lane the second
           static_assert(EPI == EPI_SWIGLU, "two matrices: gate and up");
           const bool up_lane = lane >= 16;
 #pragma unroll
-          for (int j = 0; j < 8; ++j) {
+          for (int j = 0; j < TURN / 2; ++j) {
             const float give = __uint_as_float(up_lane ? a[2 * j] : a[2 * j + 1]);
             const float keep = __uint_as_float(up_lane ? a[2 * j + 1] : a[2 * j]);
             const float got = __shfl_xor_sync(0xffffffffu, give, 16);
-            const int pi = j0 + 2 * j + (up_lane ? 1 : 0);
-            const float v = swiglu32(up_lane ? got : keep, up_lane ? keep : got, limit);
-            if (pi < cnt && col < N) static_cast<uint16_t*>(out)[(size_t)pair[pi] * N + col] = to16<F16>(v);
+            reinterpret_cast<uint16_t*>(turn)[2 * j * COLS_W + lane] =
+                to16<F16>(swiglu32(up_lane ? got : keep, up_lane ? keep : got, limit));
           }
         } else {
 #pragma unroll
-          for (int j = 0; j < 16; ++j) {
-            if (j0 + j >= cnt || col >= N) continue;
+          for (int j = 0; j < TURN; ++j) {
             float v = __uint_as_float(a[j]);
-            const size_t o = (size_t)pair[j0 + j] * N + col;
-            if constexpr (EPI == EPI_RELU2) {
-              v = v > 0.f ? v * v : v != v ? v : 0.f;                      // NaN stays NaN
-            }
-            if constexpr (EPI == EPI_F32) static_cast<float*>(out)[o] = v;
-            else static_cast<uint16_t*>(out)[o] = to16<F16>(v);
+            if constexpr (EPI == EPI_RELU2) v = v > 0.f ? v * v : v != v ? v : 0.f;      // NaN stays NaN
+            if constexpr (EPI == EPI_F32) reinterpret_cast<float*>(turn)[j * COLS_W + lane] = v;
+            else reinterpret_cast<uint16_t*>(turn)[j * COLS_W + lane] = to16<F16>(v);
           }
         }
+        __syncwarp();
+        if (wide) {
+#pragma unroll
+          for (int i = 0; i < TURN * CHUNKS / 32; ++i) {
+            const int at = i * 32 + lane, p = pair[j0 + at / CHUNKS], c = c0 + at % CHUNKS * (16 / OUT);
+            const uint4 v = *reinterpret_cast<const uint4*>(turn + at * 16);
+            if (p >= 0 && c < N) *reinterpret_cast<uint4*>(static_cast<uint8_t*>(out) + ((size_t)p * N + c) * OUT) = v;
+          }
+        } else {
+          for (int at = lane; at < TURN * COLS_W; at += 32) {
+            const int p = pair[j0 + at / COLS_W], c = c0 + at % COLS_W;
+            if (p < 0 || c >= N) continue;
+            if constexpr (EPI == EPI_F32) static_cast<float*>(out)[(size_t)p * N + c] = reinterpret_cast<const float*>(turn)[at];
+            else static_cast<uint16_t*>(out)[(size_t)p * N + c] = reinterpret_cast<const uint16_t*>(turn)[at];
+          }
+        }
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) {
+        if constexpr (CG == 1) mbar_arrive(acc_free + (n & 1));
+        else mbar_arrive_leader(acc_free + (n & 1));
       }
     }
   }
   pdl_launch_dependents();
   tc_fence_before();
   __syncthreads();
-  if (warp == 4) tmem_dealloc(tmem_base, MAXP);
+  if constexpr (CG == 2) {                                                 // nobody arrives on this CTA's barriers any more
+    cluster_arrive();
+    cluster_wait();
+  }
+  if (warp == G16_MMA_WARP) g16_dealloc<CG>(tmem_base, 2 * SH::ACC_COLS);
 }
 
-template <int M, int EPI, bool F16, int MAXP>
-int launch_g16(const void* x, int64_t x_stride, int slots, const void* w, int k, int n, const int* items, const int* counts,
-               const int* members, void* out, float limit, int64_t max_items, cudaStream_t stream) {
-  using SM = G16Smem<MAXP>;
-  auto* kern = g16_kernel<M, EPI, F16, MAXP>;
+// The driver's encoder of tensor maps, looked up once.
+inline PFN_cuTensorMapEncodeTiled_v12000 tensor_map_encoder() {
+  static PFN_cuTensorMapEncodeTiled_v12000 fn = [] {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult got;
+    if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &p, 12000, cudaEnableDefault, &got) != cudaSuccess ||
+        got != cudaDriverEntryPointSuccess)
+      p = nullptr;
+    return reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(p);
+  }();
+  return fn;
+}
+
+template <int CG, int M, int EPI, bool F16, int MAXP, int RU>
+int launch_g16(const void* x, int64_t x_stride, int64_t x_rows, int slots, const void* w, int experts, int k, int n, const int* items,
+               const int* counts, const int* members, void* out, float limit, int64_t max_items, cudaStream_t stream) {
+  using SH = G16Shape<CG, MAXP, RU>;
+  auto* kern = g16_kernel<CG, M, EPI, F16, MAXP, RU>;
   static bool configured[64] = {false};
   int dev = 0;
   TFB_CUDA(cudaGetDevice(&dev), "experts16: cudaGetDevice");
   if (dev < 0 || dev >= 64) return fail(TFB_ERR_ARG, "experts16: device index %d out of range", dev);
   if (!configured[dev]) {
-    TFB_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, SM::TOTAL),
+    TFB_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, SH::TOTAL),
              "experts16: shared memory opt-in");
     configured[dev] = true;
   }
-  const int64_t grid = max_items * ((w16_rows(M, n) + W16_ROWS - 1) / W16_ROWS);
-  if (grid >= (int64_t(1) << 31)) return fail(TFB_ERR_ARG, "experts16: too many units");
-  return check_cuda(launch(kern, dim3((unsigned)grid), dim3(G16_THREADS), (size_t)SM::TOTAL, stream,
-                           static_cast<const uint16_t*>(x), x_stride, slots, static_cast<const uint8_t*>(w), k, n, items,
-                           counts, members, out, limit),
+  auto* encode = tensor_map_encoder();
+  if (encode == nullptr) return fail(TFB_ERR_CUDA, "experts16: the driver has no cuTensorMapEncodeTiled");
+  CUtensorMap map;
+  const cuuint64_t sizes[2] = {(cuuint64_t)k, (cuuint64_t)x_rows}, strides[1] = {(cuuint64_t)x_stride * 2};
+  const cuuint32_t box[2] = {W16_K, 1}, steps[2] = {1, 1};
+  const CUresult rc = encode(&map, F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2,
+                             const_cast<void*>(x), sizes, strides, box, steps, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                             CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (rc != CUDA_SUCCESS) return fail(TFB_ERR_CUDA, "experts16: no tensor map of x (%d)", (int)rc);
+  CUtensorMap wmap = map;                                                  // read by pairs of CTAs alone
+  if (CG == 2) {
+    const int64_t lines = (int64_t)experts * w16_rows(M, n) * w16_kblocks(k);
+    if (lines >= (int64_t(1) << 31)) return fail(TFB_ERR_ARG, "experts16: weights of 2^31 lines of 64 inputs or more");
+    const cuuint64_t w_sizes[2] = {W16_K, (cuuint64_t)lines}, w_strides[1] = {W16_K * 2};
+    const cuuint32_t w_box[2] = {W16_K, W16_ROWS};
+    const CUresult wrc = encode(&wmap, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(w), w_sizes, w_strides, w_box, steps,
+                                CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (wrc != CUDA_SUCCESS) return fail(TFB_ERR_CUDA, "experts16: no tensor map of the weights (%d)", (int)wrc);
+  }
+  const int64_t units = max_items * ((w16_rows(M, n) + CG * RU - 1) / (CG * RU));
+  if (units >= (int64_t(1) << 30)) return fail(TFB_ERR_ARG, "experts16: too many units");
+  const int64_t most = sm_count() / CG, walkers = units < most ? units : most;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(walkers * CG));
+  cfg.blockDim = dim3(G16_THREADS);
+  cfg.dynamicSmemBytes = SH::TOTAL;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = CG;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = CG == 1 ? attr + 1 : attr;
+  cfg.numAttrs = (CG == 1 ? 0 : 1) + (g_use_pdl ? 1 : 0);
+  return check_cuda(cudaLaunchKernelEx(&cfg, kern, map, wmap, slots, static_cast<const uint8_t*>(w), k, n, items, counts, members,
+                                       out, limit),
                     "experts16");
+}
+
+// Rows a unit takes: 128 unless 64 or 32 leave the busiest CTA a tenth fewer rows.
+inline int g16_unit_rows(int64_t items, int rows) {
+  int best = 128;
+  int64_t most = 0;
+  for (int ru = 128; ru >= 32; ru /= 2) {
+    const int64_t units = items * ((rows + ru - 1) / ru), load = (units + sm_count() - 1) / sm_count() * ru;
+    if (ru == 128 || load * 10 <= most * 9) {
+      best = ru;
+      most = load;
+    }
+  }
+  return best;
 }
 
 }  // namespace tfb
@@ -331,7 +629,7 @@ extern "C" int tfb_unpack16(const void* packed, void* m0, void* m1, int experts,
 // when slots is 0.  out: [P, n], row p of pair p.  max_items: an upper bound of the plan's items, which hold at most `tile`
 // pairs (1..256).
 extern "C" int tfb_experts16(int epi, int fp16, const void* x, int64_t x_stride, int64_t x_rows, int slots, const void* w,
-                             int k, int n, const int32_t* items, const int32_t* counts, const int32_t* members, void* out,
+                             int experts, int k, int n, const int32_t* items, const int32_t* counts, const int32_t* members, void* out,
                              float limit, int64_t max_items, int tile, void* stream) {
   TFB_REQUIRE(x && w && items && counts && members && out, "experts16: null pointer");
   TFB_REQUIRE(k >= 8 && k % 8 == 0 && k < (1 << 24) && n >= 1 && n < (1 << 24),
@@ -339,15 +637,21 @@ extern "C" int tfb_experts16(int epi, int fp16, const void* x, int64_t x_stride,
   TFB_REQUIRE(aligned16(x) && x_stride % 8 == 0 && x_stride >= k && x_rows >= 0 && x_rows < (int64_t(1) << 31),
               "experts16: x rows of K inputs, 16-byte aligned");
   TFB_REQUIRE(aligned16(w), "experts16: w must be 16-byte aligned");
-  TFB_REQUIRE(slots >= 0 && max_items >= 0, "experts16: bad slots or item count");
+  TFB_REQUIRE(slots >= 0 && max_items >= 0 && experts >= 1, "experts16: bad slots, item or expert count");
   TFB_REQUIRE(tile >= 1 && tile <= G16_MAXP, "experts16: items of 1..%d pairs, not %d", G16_MAXP, tile);
   if (max_items == 0 || x_rows == 0) return TFB_OK;
   auto st = static_cast<cudaStream_t>(stream);
-#define TFB_G16(EPI_, M_, F16_)                                                                                             \
-  return tile <= 64 ? launch_g16<M_, EPI_, F16_, 64>(x, x_stride, slots, w, k, n, items, counts, members, out, limit,        \
-                                                     max_items, st)                                                         \
-                    : launch_g16<M_, EPI_, F16_, 256>(x, x_stride, slots, w, k, n, items, counts, members, out, limit,       \
-                                                      max_items, st)
+#define TFB_G16_AT(CG_, EPI_, M_, F16_, MAXP_, RU_) \
+  return launch_g16<CG_, M_, EPI_, F16_, MAXP_, RU_>(x, x_stride, x_rows, slots, w, experts, k, n, items, counts, members, out, limit, max_items, st)
+#define TFB_G16(EPI_, M_, F16_)                                   \
+  do {                                                            \
+    if (tile > 128) TFB_G16_AT(2, EPI_, M_, F16_, 256, 128);      \
+    if (tile > 32) TFB_G16_AT(2, EPI_, M_, F16_, 128, 128);       \
+    const int ru = g16_unit_rows(max_items, w16_rows(M_, n));     \
+    if (ru == 128) TFB_G16_AT(1, EPI_, M_, F16_, 32, 128);        \
+    if (ru == 64) TFB_G16_AT(1, EPI_, M_, F16_, 32, 64);          \
+    TFB_G16_AT(1, EPI_, M_, F16_, 32, 32);                        \
+  } while (0)
 #define TFB_G16_EPI(EPI_, M_)          \
   if (epi == EPI_) {                   \
     if (fp16) TFB_G16(EPI_, M_, true); \
@@ -355,6 +659,7 @@ extern "C" int tfb_experts16(int epi, int fp16, const void* x, int64_t x_stride,
   }
   TFB_G16_EPI(EPI_F32, 1) TFB_G16_EPI(EPI_RELU2, 1) TFB_G16_EPI(EPI_SWIGLU, 2) TFB_G16_EPI(EPI_BF16, 1)
 #undef TFB_G16
+#undef TFB_G16_AT
 #undef TFB_G16_EPI
   return fail(TFB_ERR_ARG, "experts16: no kernel for epilogue %d", epi);
 }

@@ -18,8 +18,7 @@ from . import experts as grouped
 
 DTYPES = (torch.bfloat16, torch.float16)
 ITEM = 256               # pairs an item holds at most: the tensor-core tile's N
-SMALL_ITEM = 64          # the same in the kernel's build for few pairs an expert
-SMALL_ITEM_FROM = 32     # pairs an expert on average up to which that build is used
+SMALL_ITEMS = ((16, 32), (96, 128))     # up to so many pairs an expert on average: items of so many
 
 
 def _rows(mats: int, n: int) -> int:
@@ -109,7 +108,10 @@ def unpack(ex: Experts16) -> tuple[list[torch.Tensor], torch.Tensor]:
 def item_pairs(pairs: int, experts: int) -> int:
     """Pairs an item of a plan holds; a pair's bits do not depend on it."""
 
-    return SMALL_ITEM if pairs <= SMALL_ITEM_FROM * experts else ITEM
+    for most, item in SMALL_ITEMS:
+        if pairs <= most * experts:
+            return item
+    return ITEM
 
 
 class Plan(grouped.Plan):
@@ -141,7 +143,7 @@ def _run(epi: int, x: torch.Tensor, slots: int, w: torch.Tensor, k: int, n: int,
         raise ValueError(f"{rows} rows do not fit a plan of {plan.rows}")
     with _lib.on(x.device):
         _lib.call("tfb_experts16", epi, int(w.dtype == torch.float16), x.data_ptr(), x.stride(0) if x.shape[0] > 1 else k,
-                  need, slots, w.data_ptr(), k, n, plan.items.data_ptr(), plan.counts.data_ptr(), plan.members.data_ptr(),
+                  need, slots, w.data_ptr(), w.shape[0], k, n, plan.items.data_ptr(), plan.counts.data_ptr(), plan.members.data_ptr(),
                   out.data_ptr(), float(limit), grouped.max_items(pairs, plan.experts, plan.tile), plan.tile,
                   _lib.stream(x.device))
 

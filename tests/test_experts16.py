@@ -13,14 +13,14 @@ BF, HF = torch.bfloat16, torch.float16
 def test_entry_points_refuse_bad_arguments_before_any_launch():
     from tensorfold_b200 import _lib
 
-    g16 = [2, 0, 16, 64, 8, 2, 16, 64, 32, 16, 16, 16, 16, 0.0, 4, 64, 0]
+    g16 = [2, 0, 16, 64, 8, 2, 16, 3, 64, 32, 16, 16, 16, 16, 0.0, 4, 64, 0]
     cases = [("tfb_pack16", (0, 0, 16, 1, 16, 64, 0), "null pointer"),
              ("tfb_pack16", (16, 0, 16, 1, 16, 60, 0), "does not pack"),
              ("tfb_pack16", (16, 24, 16, 1, 16, 64, 0), "16-byte aligned"),
              ("tfb_unpack16", (16, 16, 0, 0, 16, 64, 0), "does not pack")]
-    for at, value, why in ((2, 0, "null pointer"), (7, 60, "multiples of 8"), (8, 0, "columns"), (3, 56, "x rows"),
-                           (3, 68, "x rows"), (2, 24, "16-byte aligned"), (5, -1, "bad slots"), (15, 257, "items of 1..256"),
-                           (15, 0, "items of 1..256"), (0, 4, "no kernel for epilogue 4"), (4, 1 << 31, "x rows")):
+    for at, value, why in ((2, 0, "null pointer"), (8, 60, "multiples of 8"), (9, 0, "columns"), (3, 56, "x rows"),
+                           (3, 68, "x rows"), (2, 24, "16-byte aligned"), (5, -1, "bad slots"), (16, 257, "items of 1..256"),
+                           (16, 0, "items of 1..256"), (7, 0, "expert count"), (0, 4, "no kernel for epilogue 4"), (4, 1 << 31, "x rows")):
         bad = list(g16)
         bad[at] = value
         cases.append(("tfb_experts16", tuple(bad), why))
@@ -40,8 +40,8 @@ def test_entry_points_refuse_bad_arguments_before_any_launch():
 def test_calls_without_work_launch_nothing():
     from tensorfold_b200 import _lib
 
-    _lib.call("tfb_experts16", 0, 0, 16, 64, 0, 2, 16, 64, 32, 16, 16, 16, 16, 0.0, 4, 64, 0)
-    _lib.call("tfb_experts16", 0, 0, 16, 64, 8, 2, 16, 64, 32, 16, 16, 16, 16, 0.0, 0, 64, 0)
+    _lib.call("tfb_experts16", 0, 0, 16, 64, 0, 2, 16, 3, 64, 32, 16, 16, 16, 16, 0.0, 4, 64, 0)
+    _lib.call("tfb_experts16", 0, 0, 16, 64, 8, 2, 16, 3, 64, 32, 16, 16, 16, 16, 0.0, 0, 64, 0)
     _lib.call("tfb_adapters", 0, 16, 64, 16, 16, 16, 16, 64, 32, 16, 0, 2, 0, 0, 0, 0, 16, 0, 32, 32, 1, 32, 0)
 
 
@@ -63,9 +63,8 @@ def test_weights_that_do_not_fit_together_are_refused():
 def test_item_sizes():
     from tensorfold_b200 import experts16
 
-    assert experts16.item_pairs(8, 128) == experts16.SMALL_ITEM
-    assert experts16.item_pairs(32 * 128 + 1, 128) == experts16.ITEM
-    assert experts16.Plan(4, 2, 8, "cpu").tile == experts16.SMALL_ITEM
+    assert experts16.item_pairs(8, 128) < experts16.item_pairs(128 * 1024, 128) == experts16.ITEM
+    assert experts16.Plan(4, 2, 8, "cpu").tile == experts16.item_pairs(8, 8)
 
 
 def test_cpu_tensors_are_refused():
