@@ -73,33 +73,35 @@ unpack16_kernel(const uint4* packed, uint8_t* m0, uint8_t* m1, int mats, int n, 
 // Persistent: the CTAs (CG = 1), or pairs of CTAs whose tensor cores work as one (CG = 2), walk units = (item, CG * RU rows
 // of its expert's weights).  A CTA's roles run apart, each through all of its units, so that the copies of the next unit
 // travel while the last one is finished:
-//   warp 5     the weights' bulk copies: RU rows;  warps 6-9 the pairs' input rows by TMA gathers (four rows an instruction,
-//              zeros behind the last input), of a pair of CTAs each one half; both into a ring of stages of 128 / RU blocks
-//              of 64 inputs, 16 KB of weights each;
-//   warp 4     one lane (of a pair's first CTA, on whose barriers both CTAs' copies count) issues tcgen05.mma (M = 128 CG, N =
-//              pairs) into one of two accumulators in tensor memory;
-//   warps 0-3  read the other accumulator, apply the activation and store the pairs' rows: through shared memory, where a
-//              lane's one column of many pairs becomes 16 bytes of a pair's row.  (Stored from the registers, 2 bytes a
-//              lane, a unit of 256 pairs took 14 us to finish where its products take 3 to 9.)
+//   one warp   the weights' bulk copies: RU rows;  four or eight warps the pairs' input rows by TMA gathers (four rows an
+//              instruction, zeros behind the last input), of a pair of CTAs each one half; both into a ring of stages of
+//              128 / RU blocks of 64 inputs, 16 KB of weights each;
+//   one warp   (of a pair's first CTA, on whose barriers both CTAs' copies count) issues tcgen05.mma (M = 128 CG, N = pairs)
+//              into one of two accumulators in tensor memory;
+//   four or eight warps  read the other accumulator, apply the activation and store the pairs' rows: through shared memory,
+//              where a lane's one column of many pairs becomes 16 bytes of a pair's row.  (Stored from the registers, 2
+//              bytes a lane, a unit of 256 pairs took 14 us to finish where its products take 3 to 9.)
+// A role's loop runs in all lanes of its warp with one lane elected for the issue: addresses and descriptors stay in uniform
+// registers.  (In a loop of lane 0 alone an MMA took 80 cycles to issue, and at few pairs that was the kernel's time.)
 constexpr int G16_MAXP = 256;                      // pairs an item may hold (MMA N)
-constexpr int G16_B_WARPS = 4;
-constexpr int G16_MMA_WARP = 4, G16_A_WARP = 5, G16_B_WARP = 6;
-constexpr int G16_THREADS = (G16_B_WARP + G16_B_WARPS) * 32;
 
 template <int CG, int MAXP, int RU>
 struct G16Shape {
+  static constexpr int EPI_WARPS = 4 * CG, B_WARPS = 4 * CG;               // finishing, gathering
+  static constexpr int MMA_WARP = EPI_WARPS, A_WARP = MMA_WARP + 1, B_WARP = A_WARP + 1;
+  static constexpr int THREADS = (B_WARP + B_WARPS) * 32;
   static constexpr int KPS = W16_ROWS / RU;                                // blocks of 64 inputs a stage
   static constexpr int A_BYTES = W16_ROWS * 128, B_BLOCK = MAXP / CG * 128, B_BYTES = KPS * B_BLOCK;
   static constexpr int STAGE = A_BYTES + B_BYTES;
-  static constexpr int STAGES = (214 * 1024 / STAGE) < 10 ? (214 * 1024 / STAGE) : 10;
+  static constexpr int STAGES = (206 * 1024 / STAGE) < 10 ? (206 * 1024 / STAGE) : 10;
   static constexpr int TABLE_OFFSET = STAGES * STAGE;                      // int pair[2][MAXP]
   static constexpr int TURN_OFFSET = TABLE_OFFSET + 2 * MAXP * 4;          // the finishing warps' rows: 2 KB each
-  static constexpr int BAR_OFFSET = TURN_OFFSET + 4 * 2048;
+  static constexpr int BAR_OFFSET = TURN_OFFSET + EPI_WARPS * 2048;
   static constexpr int TMEM_OFFSET = BAR_OFFSET + (2 * STAGES + 4) * 8;
   static constexpr int TOTAL = TMEM_OFFSET + 16 + 1024;                    // + slack to align the tiles to 1024 bytes
   static constexpr int ACC_COLS = MAXP;                                    // tensor memory: two accumulators
   static constexpr int STEP = 16 * CG;                                     // N is a multiple of it
-  static constexpr int LANES = MAXP / CG / 4 / G16_B_WARPS;                // lanes of a gathering warp with a group of rows
+  static constexpr int LANES = (MAXP / CG / 4 + B_WARPS - 1) / B_WARPS;                // lanes of a gathering warp with a group of rows
   static_assert(TOTAL <= 227 * 1024, "one CTA's shared memory");
   static_assert(ACC_COLS >= 32 && 2 * ACC_COLS <= 512 && LANES >= 1 && LANES <= 32, "tensor memory; the gathers");
   static_assert((KPS - 1) * RU * 128 + A_BYTES <= STAGE, "an operand of 128 rows of which RU are this unit's stays in its stage");
@@ -202,12 +204,14 @@ __device__ __forceinline__ void mbar_arrive_leader(uint64_t* bar) {
   asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];\n" ::"r"(leader_addr(bar)) : "memory");
 }
 
-// mbar_wait for a barrier on which the other CTA of the pair arrives too.  (Once a unit: with this scope a wait costs half a
-// microsecond, which at every stage was most of the kernel's time.)
-__device__ __forceinline__ bool mbar_wait_cluster(uint64_t* bar, uint32_t parity) {
-  if (!mbar_wait(bar, parity)) return false;
-  asm volatile("fence.acq_rel.cluster;\n" ::: "memory");
-  return true;
+__device__ __forceinline__ void mbar_expect_tx_at(uint32_t bar, uint32_t bytes) {
+  asm volatile("mbarrier.arrive.expect_tx.relaxed.cluster.shared::cluster.b64 _, [%0], %1;\n" ::"r"(bar), "r"(bytes) : "memory");
+}
+
+__device__ __forceinline__ bool elect_one() {
+  uint32_t on;
+  asm volatile("{\n.reg .pred p;\nelect.sync _|p, 0xffffffff;\nselp.u32 %0, 1, 0, p;\n}\n" : "=r"(on));
+  return on != 0;
 }
 
 // Four rows' 64 inputs from column `col` on into 512 bytes of a swizzled operand tile; zeros behind the map's columns.  `bar`:
@@ -266,12 +270,12 @@ struct RingAt {                                     // a walk around the ring of
 // Every role reads what it needs of the plan one unit ahead: behind the last copy of a unit the chain item -> members ->
 // rows took 2 us in which the ring ran dry.
 template <int CG, int M, int EPI, bool F16, int MAXP, int RU>
-__global__ void __launch_bounds__(G16_THREADS, 1)
+__global__ void __launch_bounds__(G16Shape<CG, MAXP, RU>::THREADS, 1)
 g16_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ CUtensorMap wmap, int slots, const uint8_t* __restrict__ W, int K, int N,
            const int* __restrict__ items, const int* __restrict__ counts, const int* __restrict__ members,
            void* __restrict__ out, float limit) {
   using SH = G16Shape<CG, MAXP, RU>;
-  constexpr int STAGES = SH::STAGES, KPS = SH::KPS;
+  constexpr int STAGES = SH::STAGES, KPS = SH::KPS, B_WARPS = SH::B_WARPS;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   int* table = reinterpret_cast<int*>(smem + SH::TABLE_OFFSET);
@@ -280,7 +284,7 @@ g16_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ CUt
   uint64_t* acc_full = empty + STAGES;                                     // [2] a unit's sums are complete
   uint64_t* acc_free = acc_full + 2;                                       // [2] and have been read
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + SH::TMEM_OFFSET);
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
   const int cta = CG == 1 ? 0 : (int)cluster_rank();                       // of the pair; 0 issues the MMAs
   const int rows = w16_rows(M, N), KB = w16_kblocks(K), nct = (rows + CG * RU - 1) / (CG * RU);
   const int fills = (KB + KPS - 1) / KPS;                                  // stages a unit takes
@@ -288,19 +292,19 @@ g16_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ CUt
 
   if (tid == 0) {
     for (int s = 0; s < STAGES; ++s) {
-      // every warp that waits for `empty` arrives here or has copies that do: one that had no part in a stage could fall a
-      // round behind and mistake the barrier's phase
-      mbar_init(full + s, 1 + G16_B_WARPS);
+      // every warp that waits for `empty` arrives here: one that had no part in a stage could fall a round behind and mistake
+      // the barrier's phase
+      mbar_init(full + s, CG * (1 + B_WARPS));
       mbar_init(empty + s, 1);
     }
     for (int s = 0; s < 2; ++s) {
       mbar_init(acc_full + s, 1);
-      mbar_init(acc_free + s, 4 * CG);
+      mbar_init(acc_free + s, SH::EPI_WARPS * CG);
     }
     mbar_fence_init();
     fence_async_smem();
   }
-  if (warp == G16_MMA_WARP) g16_alloc<CG>(tmem_slot, 2 * SH::ACC_COLS);
+  if (warp == SH::MMA_WARP) g16_alloc<CG>(tmem_slot, 2 * SH::ACC_COLS);
   pdl_wait();
   after_wait(items, counts, members);
   tc_fence_before();
@@ -311,45 +315,48 @@ g16_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ CUt
   }
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
-  const int units = ld_dep(counts) * nct;
+  const int units = __shfl_sync(0xffffffffu, ld_dep(counts), 0) * nct;
   bool ok = true;
   auto item = [&](int u) { return min(u, units - 1) / nct; };              // of the next unit, or any where there is none
 
   if (units == 0) {
-  } else if (warp == G16_A_WARP) {
-    if (lane == 0) {
-      RingAt at;
-      int e = ld_dep(items + 3 * item(u0));
-      for (int u = u0; u < units && ok; u += du) {
-        const int r0 = ((u - u / nct * nct) * CG + cta) * RU;
-        const int t0 = CG == 2 && r0 >= rows ? 0 : r0 / W16_ROWS * W16_ROWS;   // a second CTA without rows multiplies any
-        const int rt = min(W16_ROWS, rows - t0), ru = min(RU, rows - r0);
-        const uint8_t* src = W + ((size_t)e * rows + t0) * KB * 128 + (r0 - t0) * 128;
-        const int row = (e * rows + t0) * KB;
-        e = ld_dep(items + 3 * item(u + du));
-        for (int f = 0; f < fills; ++f) {
-          ok = mbar_wait(empty + at.s, at.ph ^ 1);                         // the ring's first round finds every stage free
-          if (!ok) break;
-          uint8_t* dst = smem + at.s * SH::STAGE;
+  } else if (warp == SH::A_WARP) {
+    RingAt at;
+    int e = ld_dep(items + 3 * item(u0));
+    for (int u = u0; u < units && ok; u += du) {
+      const int r0 = ((u - u / nct * nct) * CG + cta) * RU;
+      const int t0 = CG == 2 && r0 >= rows ? 0 : r0 / W16_ROWS * W16_ROWS;     // a second CTA without rows multiplies any
+      const int rt = min(W16_ROWS, rows - t0), ru = min(RU, rows - r0);
+      const int ee = __shfl_sync(0xffffffffu, e, 0);
+      const uint8_t* src = W + ((size_t)ee * rows + t0) * KB * 128 + (r0 - t0) * 128;
+      const int row = (ee * rows + t0) * KB;
+      e = ld_dep(items + 3 * item(u + du));
+      for (int f = 0; f < fills; ++f) {
+        ok = mbar_wait_warp(empty + at.s, at.ph ^ 1);                      // the ring's first round finds every stage free
+        if (!ok) break;
+        uint8_t* dst = smem + at.s * SH::STAGE;
+        if (elect_one()) {
           if constexpr (CG == 1) {
             const int nkb = min(KPS, KB - f * KPS);
             mbar_expect_tx(full + at.s, (uint32_t)(nkb * ru) * 128);
             for (int b = 0; b < nkb; ++b)
               bulk_g2s(dst + b * (RU * 128), src + (size_t)(f * KPS + b) * rt * 128, ru * 128, full + at.s);
           } else {                                                         // 128 rows: behind a shorter tile's, the next block's
-            if (cta == 0) mbar_expect_tx(full + at.s, 2 * SH::A_BYTES);
-            tma_rows_pair(dst, &wmap, row + f * rt, leader_addr(full + at.s));
+            const uint32_t bar = leader_addr(full + at.s);
+            mbar_expect_tx_at(bar, SH::A_BYTES);
+            tma_rows_pair(dst, &wmap, row + f * rt, bar);
           }
-          at.next(STAGES);
         }
+        __syncwarp();
+        at.next(STAGES);
       }
-      if (!ok) at.drain(full, STAGES, cta == 0);
     }
+    if (!ok) at.drain(full, STAGES, cta == 0);
     __syncwarp();
-  } else if (warp >= G16_B_WARP) {
-    // Lane l of warp w takes group l * B_WARPS + w of four rows.  (One lane's gathers follow one another every 130 ns, those
-    // of a warp's lanes every 41.)
-    const int g = lane * G16_B_WARPS + warp - G16_B_WARP;
+  } else if (warp >= SH::B_WARP) {
+    // Lane l of warp w takes group l * B_WARPS + w of four rows.  A warp's gathers follow one another every 130 cycles,
+    // whichever lanes issue them, hence the warps.
+    const int g = lane * B_WARPS + warp - SH::B_WARP;
     RingAt at;
     int4 next;
     int next_cnt;
@@ -370,16 +377,20 @@ g16_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ CUt
     for (int u = u0; u < units && ok; u += du) {
       int4 r = next;
       if (slots) r = make_int4(r.x / slots, r.y / slots, r.z / slots, r.w / slots);
-      const int groups = (next_cnt + SH::STEP - 1) / SH::STEP * SH::STEP / CG / 4;     // of this CTA: a multiple of B_WARPS
+      const int groups = (next_cnt + SH::STEP - 1) / SH::STEP * SH::STEP / CG / 4;     // of this CTA
+      const int here = max(0, (groups - (warp - SH::B_WARP) + B_WARPS - 1) / B_WARPS);   // of this warp
       fetch(u + du);
       for (int f = 0; f < fills; ++f) {
         ok = mbar_wait_warp(empty + at.s, at.ph ^ 1);
         if (!ok) break;
         const int nkb = min(KPS, KB - f * KPS);
         uint8_t* dst = smem + at.s * SH::STAGE + SH::A_BYTES + g * 512;
-        if (lane == 0 && cta == 0) mbar_expect_tx(full + at.s, (uint32_t)(CG * nkb * (groups / G16_B_WARPS)) * 512);
-        __syncwarp();
         const uint32_t bar = CG == 1 ? smem_addr(full + at.s) : leader_addr(full + at.s);
+        if (lane == 0) {
+          if constexpr (CG == 1) mbar_expect_tx(full + at.s, (uint32_t)(nkb * here) * 512);
+          else mbar_expect_tx_at(bar, (uint32_t)(nkb * here) * 512);
+        }
+        __syncwarp();
         if (lane < SH::LANES && g < groups)
           for (int b = 0; b < nkb; ++b) tma_gather4<CG>(dst + b * SH::B_BLOCK, &xmap, (f * KPS + b) * W16_K, r, bar);
         __syncwarp();
@@ -388,51 +399,54 @@ g16_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ CUt
     }
     if (!ok) at.drain(full, STAGES, cta == 0);
     __syncwarp();
-  } else if (warp == G16_MMA_WARP) {
-    if (lane == 0 && cta == 0) {
+  } else if (warp == SH::MMA_WARP) {
+    if (cta == 0) {
       const uint64_t a0 = umma_desc(smem_addr(smem)), b0 = umma_desc(smem_addr(smem + SH::A_BYTES));
       RingAt at;
       int n = 0;                                                           // the CTA's n-th unit
       int next_cnt = ld_dep(items + 3 * item(u0) + 2);
       for (int u = u0; u < units && ok; u += du, ++n) {
-        const int cnt = min(next_cnt, MAXP);
+        const int cnt = min(__shfl_sync(0xffffffffu, next_cnt, 0), MAXP);
         next_cnt = ld_dep(items + 3 * item(u + du) + 2);
         const uint32_t idesc = g16_idesc<CG, F16>((cnt + SH::STEP - 1) / SH::STEP * SH::STEP);
         const uint32_t acc = tmem_base + (n & 1) * SH::ACC_COLS;
-        ok = CG == 1 ? mbar_wait(acc_free + (n & 1), ((n >> 1) & 1) ^ 1) : mbar_wait_cluster(acc_free + (n & 1), ((n >> 1) & 1) ^ 1);
+        ok = mbar_wait_warp(acc_free + (n & 1), ((n >> 1) & 1) ^ 1);
         if (!ok) break;
+        if constexpr (CG == 2) asm volatile("fence.acq_rel.cluster;\n" ::: "memory");   // the other CTA's arrivals
         tc_fence_after();
         for (int f = 0; f < fills; ++f) {
-          ok = mbar_wait(full + at.s, at.ph);
+          ok = mbar_wait_warp(full + at.s, at.ph);
           if (!ok) break;
           tc_fence_after();
           const int nkb = min(KPS, KB - f * KPS);
-          for (int b = 0; b < nkb; ++b) {
-            const uint64_t ad = a0 + (uint32_t)((at.s * SH::STAGE + b * (RU * 128)) >> 4);
-            const uint64_t bd = b0 + (uint32_t)((at.s * SH::STAGE + b * SH::B_BLOCK) >> 4);
+          if (elect_one()) {
+            for (int b = 0; b < nkb; ++b) {
+              const uint64_t ad = a0 + (uint32_t)((at.s * SH::STAGE + b * (RU * 128)) >> 4);
+              const uint64_t bd = b0 + (uint32_t)((at.s * SH::STAGE + b * SH::B_BLOCK) >> 4);
 #pragma unroll
-            for (int ks = 0; ks < 4; ++ks) umma_ss<CG>(acc, ad + 2 * ks, bd + 2 * ks, idesc, (f | b | ks) ? 1u : 0u);
+              for (int ks = 0; ks < 4; ++ks) umma_ss<CG>(acc, ad + 2 * ks, bd + 2 * ks, idesc, (f | b | ks) ? 1u : 0u);
+            }
+            g16_commit<CG>(empty + at.s);
+            if (f == fills - 1) g16_commit<CG>(acc_full + (n & 1));
           }
-          g16_commit<CG>(empty + at.s);
+          __syncwarp();
           at.next(STAGES);
         }
-        if (ok) g16_commit<CG>(acc_full + (n & 1));
       }
     }
-    __syncwarp();
   } else {
     // ---- the finishing warps: tensor-memory lane = weight row, column = pair ----
-    const int q = warp;
-    uint8_t* turn = smem + SH::TURN_OFFSET + q * 2048;
+    const int q = warp & 3, part = warp >> 2;                              // quarter of the lanes; share of the pairs
+    uint8_t* turn = smem + SH::TURN_OFFSET + warp * 2048;
     int n = 0;
     int first = ld_dep(items + 3 * item(u0) + 1), cnt = ld_dep(items + 3 * item(u0) + 2);
     for (int u = u0; u < units && ok; u += du, ++n) {
       const int r0 = ((u - u / nct * nct) * CG + cta) * RU, have = min(cnt, MAXP);
       int* pair = table + (n & 1) * MAXP;
-      for (int i = tid; i < ((have + 31) & ~31); i += 128) pair[i] = i < have ? ld_dep(members + first + i) : -1;
+      for (int i = tid; i < ((have + 31) & ~31); i += SH::EPI_WARPS * 32) pair[i] = i < have ? ld_dep(members + first + i) : -1;
       first = ld_dep(items + 3 * item(u + du) + 1);
       cnt = ld_dep(items + 3 * item(u + du) + 2);
-      asm volatile("bar.sync 1, 128;\n" ::: "memory");
+      asm volatile("bar.sync 1, %0;\n" ::"n"(SH::EPI_WARPS * 32) : "memory");
       ok = mbar_wait_warp(acc_full + (n & 1), (n >> 1) & 1);
       if (!ok) break;
       tc_fence_after();
@@ -443,7 +457,7 @@ g16_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ CUt
       constexpr int CHUNKS = COLS_W * OUT / 16;                            // 16-byte pieces of a pair's row
       const int c0 = r0 / M + q * COLS_W;                                  // the warp's first column
       const bool wide = ((size_t)N * OUT) % 16 == 0 && (reinterpret_cast<uintptr_t>(out) & 15) == 0;
-      for (int j0 = 0; j0 < have && q * 32 < RU && c0 < N; j0 += TURN) {
+      for (int j0 = part * TURN; j0 < have && q * 32 < RU && c0 < N; j0 += SH::EPI_WARPS / 4 * TURN) {
         uint32_t a[32];
         if constexpr (TURN == 32) tmem_ld32(taddr + j0, a);
         else tmem_ld16(taddr + j0, *reinterpret_cast<uint32_t(*)[16]>(a));
@@ -503,7 +517,7 @@ g16_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ CUt
     cluster_arrive();
     cluster_wait();
   }
-  if (warp == G16_MMA_WARP) g16_dealloc<CG>(tmem_base, 2 * SH::ACC_COLS);
+  if (warp == SH::MMA_WARP) g16_dealloc<CG>(tmem_base, 2 * SH::ACC_COLS);
 }
 
 // The driver's encoder of tensor maps, looked up once.
@@ -558,7 +572,7 @@ int launch_g16(const void* x, int64_t x_stride, int64_t x_rows, int slots, const
   const int64_t most = sm_count() / CG, walkers = units < most ? units : most;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(walkers * CG));
-  cfg.blockDim = dim3(G16_THREADS);
+  cfg.blockDim = dim3(SH::THREADS);
   cfg.dynamicSmemBytes = SH::TOTAL;
   cfg.stream = stream;
   cudaLaunchAttribute attr[2];
