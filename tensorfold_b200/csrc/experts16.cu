@@ -70,12 +70,12 @@ unpack16_kernel(const uint4* packed, uint8_t* m0, uint8_t* m1, int mats, int n, 
 }
 
 // ---- the grouped product ---------------------------------------------------------------------------------------------
-// Persistent: the CTAs (CG = 1), or pairs of CTAs whose tensor cores work as one (CG = 2), walk units = (item, CG * RU rows
-// of its expert's weights).  A CTA's roles run apart, each through all of its units, so that the copies of the next unit
+// Persistent: the CTAs (CG = 1), or pairs of CTAs whose tensor cores work as one (CG = 2), walk units = (item, 128 CG rows of
+// its expert's weights).  A CTA's roles run apart, each through all of its units, so that the copies of the next unit
 // travel while the last one is finished:
-//   one warp   the weights' bulk copies: RU rows;  four or eight warps the pairs' input rows by TMA gathers (four rows an
+//   one warp   the weights' bulk copies: 128 rows;  four or eight warps the pairs' input rows by TMA gathers (four rows an
 //              instruction, zeros behind the last input), of a pair of CTAs each one half; both into a ring of stages of
-//              128 / RU blocks of 64 inputs, 16 KB of weights each;
+//              64 inputs, 16 KB of weights each;
 //   one warp   (of a pair's first CTA, on whose barriers both CTAs' copies count) issues tcgen05.mma (M = 128 CG, N = pairs)
 //              into one of two accumulators in tensor memory;
 //   four or eight warps  read the other accumulator, apply the activation and store the pairs' rows: through shared memory,
@@ -85,13 +85,12 @@ unpack16_kernel(const uint4* packed, uint8_t* m0, uint8_t* m1, int mats, int n, 
 // registers.  (In a loop of lane 0 alone an MMA took 80 cycles to issue, and at few pairs that was the kernel's time.)
 constexpr int G16_MAXP = 256;                      // pairs an item may hold (MMA N)
 
-template <int CG, int MAXP, int RU>
+template <int CG, int MAXP>
 struct G16Shape {
   static constexpr int EPI_WARPS = 4 * CG, B_WARPS = 4 * CG;               // finishing, gathering
   static constexpr int MMA_WARP = EPI_WARPS, A_WARP = MMA_WARP + 1, B_WARP = A_WARP + 1;
   static constexpr int THREADS = (B_WARP + B_WARPS) * 32;
-  static constexpr int KPS = W16_ROWS / RU;                                // blocks of 64 inputs a stage
-  static constexpr int A_BYTES = W16_ROWS * 128, B_BLOCK = MAXP / CG * 128, B_BYTES = KPS * B_BLOCK;
+  static constexpr int A_BYTES = W16_ROWS * 128, B_BYTES = MAXP / CG * 128;
   static constexpr int STAGE = A_BYTES + B_BYTES;
   static constexpr int STAGES = (206 * 1024 / STAGE) < 10 ? (206 * 1024 / STAGE) : 10;
   static constexpr int TABLE_OFFSET = STAGES * STAGE;                      // int pair[2][MAXP]
@@ -104,8 +103,6 @@ struct G16Shape {
   static constexpr int LANES = (MAXP / CG / 4 + B_WARPS - 1) / B_WARPS;                // lanes of a gathering warp with a group of rows
   static_assert(TOTAL <= 227 * 1024, "one CTA's shared memory");
   static_assert(ACC_COLS >= 32 && 2 * ACC_COLS <= 512 && LANES >= 1 && LANES <= 32, "tensor memory; the gathers");
-  static_assert((KPS - 1) * RU * 128 + A_BYTES <= STAGE, "an operand of 128 rows of which RU are this unit's stays in its stage");
-  static_assert(CG == 1 || RU == W16_ROWS, "a pair of CTAs takes whole tiles");
 };
 
 template <bool F16>
@@ -269,13 +266,13 @@ struct RingAt {                                     // a walk around the ring of
 
 // Every role reads what it needs of the plan one unit ahead: behind the last copy of a unit the chain item -> members ->
 // rows took 2 us in which the ring ran dry.
-template <int CG, int M, int EPI, bool F16, int MAXP, int RU>
-__global__ void __launch_bounds__(G16Shape<CG, MAXP, RU>::THREADS, 1)
+template <int CG, int M, int EPI, bool F16, int MAXP>
+__global__ void __launch_bounds__(G16Shape<CG, MAXP>::THREADS, 1)
 g16_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ CUtensorMap wmap, int slots, const uint8_t* __restrict__ W, int K, int N,
            const int* __restrict__ items, const int* __restrict__ counts, const int* __restrict__ members,
            void* __restrict__ out, float limit) {
-  using SH = G16Shape<CG, MAXP, RU>;
-  constexpr int STAGES = SH::STAGES, KPS = SH::KPS, B_WARPS = SH::B_WARPS;
+  using SH = G16Shape<CG, MAXP>;
+  constexpr int STAGES = SH::STAGES, B_WARPS = SH::B_WARPS;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   int* table = reinterpret_cast<int*>(smem + SH::TABLE_OFFSET);
@@ -286,8 +283,7 @@ g16_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ CUt
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + SH::TMEM_OFFSET);
   const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
   const int cta = CG == 1 ? 0 : (int)cluster_rank();                       // of the pair; 0 issues the MMAs
-  const int rows = w16_rows(M, N), KB = w16_kblocks(K), nct = (rows + CG * RU - 1) / (CG * RU);
-  const int fills = (KB + KPS - 1) / KPS;                                  // stages a unit takes
+  const int rows = w16_rows(M, N), KB = w16_kblocks(K), nct = (rows + CG * W16_ROWS - 1) / (CG * W16_ROWS);
   const int u0 = blockIdx.x / CG, du = gridDim.x / CG;
 
   if (tid == 0) {
@@ -324,23 +320,20 @@ g16_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ CUt
     RingAt at;
     int e = ld_dep(items + 3 * item(u0));
     for (int u = u0; u < units && ok; u += du) {
-      const int r0 = ((u - u / nct * nct) * CG + cta) * RU;
-      const int t0 = CG == 2 && r0 >= rows ? 0 : r0 / W16_ROWS * W16_ROWS;     // a second CTA without rows multiplies any
-      const int rt = min(W16_ROWS, rows - t0), ru = min(RU, rows - r0);
+      const int r0 = ((u - u / nct * nct) * CG + cta) * W16_ROWS, t0 = r0 < rows ? r0 : 0;   // a second CTA without rows: any
+      const int rt = min(W16_ROWS, rows - t0);
       const int ee = __shfl_sync(0xffffffffu, e, 0);
-      const uint8_t* src = W + ((size_t)ee * rows + t0) * KB * 128 + (r0 - t0) * 128;
+      const uint8_t* src = W + ((size_t)ee * rows + t0) * KB * 128;
       const int row = (ee * rows + t0) * KB;
       e = ld_dep(items + 3 * item(u + du));
-      for (int f = 0; f < fills; ++f) {
+      for (int f = 0; f < KB; ++f) {
         ok = mbar_wait_warp(empty + at.s, at.ph ^ 1);                      // the ring's first round finds every stage free
         if (!ok) break;
         uint8_t* dst = smem + at.s * SH::STAGE;
         if (elect_one()) {
           if constexpr (CG == 1) {
-            const int nkb = min(KPS, KB - f * KPS);
-            mbar_expect_tx(full + at.s, (uint32_t)(nkb * ru) * 128);
-            for (int b = 0; b < nkb; ++b)
-              bulk_g2s(dst + b * (RU * 128), src + (size_t)(f * KPS + b) * rt * 128, ru * 128, full + at.s);
+            mbar_expect_tx(full + at.s, (uint32_t)rt * 128);
+            bulk_g2s(dst, src + (size_t)f * rt * 128, rt * 128, full + at.s);
           } else {                                                         // 128 rows: behind a shorter tile's, the next block's
             const uint32_t bar = leader_addr(full + at.s);
             mbar_expect_tx_at(bar, SH::A_BYTES);
@@ -380,19 +373,18 @@ g16_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ CUt
       const int groups = (next_cnt + SH::STEP - 1) / SH::STEP * SH::STEP / CG / 4;     // of this CTA
       const int here = max(0, (groups - (warp - SH::B_WARP) + B_WARPS - 1) / B_WARPS);   // of this warp
       fetch(u + du);
-      for (int f = 0; f < fills; ++f) {
+      for (int f = 0; f < KB; ++f) {
         ok = mbar_wait_warp(empty + at.s, at.ph ^ 1);
         if (!ok) break;
-        const int nkb = min(KPS, KB - f * KPS);
         uint8_t* dst = smem + at.s * SH::STAGE + SH::A_BYTES + g * 512;
         const uint32_t bar = CG == 1 ? smem_addr(full + at.s) : leader_addr(full + at.s);
         if (lane == 0) {
-          if constexpr (CG == 1) mbar_expect_tx(full + at.s, (uint32_t)(nkb * here) * 512);
-          else mbar_expect_tx_at(bar, (uint32_t)(nkb * here) * 512);
+          if constexpr (CG == 1) mbar_expect_tx(full + at.s, (uint32_t)here * 512);
+          else mbar_expect_tx_at(bar, (uint32_t)here * 512);
         }
         __syncwarp();
         if (lane < SH::LANES && g < groups)
-          for (int b = 0; b < nkb; ++b) tma_gather4<CG>(dst + b * SH::B_BLOCK, &xmap, (f * KPS + b) * W16_K, r, bar);
+          tma_gather4<CG>(dst, &xmap, f * W16_K, r, bar);
         __syncwarp();
         at.next(STAGES);
       }
@@ -414,20 +406,16 @@ g16_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ CUt
         if (!ok) break;
         if constexpr (CG == 2) asm volatile("fence.acq_rel.cluster;\n" ::: "memory");   // the other CTA's arrivals
         tc_fence_after();
-        for (int f = 0; f < fills; ++f) {
+        for (int f = 0; f < KB; ++f) {
           ok = mbar_wait_warp(full + at.s, at.ph);
           if (!ok) break;
           tc_fence_after();
-          const int nkb = min(KPS, KB - f * KPS);
-          if (elect_one()) {
-            for (int b = 0; b < nkb; ++b) {
-              const uint64_t ad = a0 + (uint32_t)((at.s * SH::STAGE + b * (RU * 128)) >> 4);
-              const uint64_t bd = b0 + (uint32_t)((at.s * SH::STAGE + b * SH::B_BLOCK) >> 4);
+            if (elect_one()) {
+            const uint32_t off = (uint32_t)(at.s * SH::STAGE) >> 4;
 #pragma unroll
-              for (int ks = 0; ks < 4; ++ks) umma_ss<CG>(acc, ad + 2 * ks, bd + 2 * ks, idesc, (f | b | ks) ? 1u : 0u);
-            }
+            for (int ks = 0; ks < 4; ++ks) umma_ss<CG>(acc, a0 + off + 2 * ks, b0 + off + 2 * ks, idesc, (f | ks) ? 1u : 0u);
             g16_commit<CG>(empty + at.s);
-            if (f == fills - 1) g16_commit<CG>(acc_full + (n & 1));
+            if (f == KB - 1) g16_commit<CG>(acc_full + (n & 1));
           }
           __syncwarp();
           at.next(STAGES);
@@ -441,7 +429,7 @@ g16_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ CUt
     int n = 0;
     int first = ld_dep(items + 3 * item(u0) + 1), cnt = ld_dep(items + 3 * item(u0) + 2);
     for (int u = u0; u < units && ok; u += du, ++n) {
-      const int r0 = ((u - u / nct * nct) * CG + cta) * RU, have = min(cnt, MAXP);
+      const int r0 = ((u - u / nct * nct) * CG + cta) * W16_ROWS, have = min(cnt, MAXP);
       int* pair = table + (n & 1) * MAXP;
       for (int i = tid; i < ((have + 31) & ~31); i += SH::EPI_WARPS * 32) pair[i] = i < have ? ld_dep(members + first + i) : -1;
       first = ld_dep(items + 3 * item(u + du) + 1);
@@ -457,7 +445,7 @@ g16_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ CUt
       constexpr int CHUNKS = COLS_W * OUT / 16;                            // 16-byte pieces of a pair's row
       const int c0 = r0 / M + q * COLS_W;                                  // the warp's first column
       const bool wide = ((size_t)N * OUT) % 16 == 0 && (reinterpret_cast<uintptr_t>(out) & 15) == 0;
-      for (int j0 = part * TURN; j0 < have && q * 32 < RU && c0 < N; j0 += SH::EPI_WARPS / 4 * TURN) {
+      for (int j0 = part * TURN; j0 < have && c0 < N; j0 += SH::EPI_WARPS / 4 * TURN) {
         uint32_t a[32];
         if constexpr (TURN == 32) tmem_ld32(taddr + j0, a);
         else tmem_ld16(taddr + j0, *reinterpret_cast<uint32_t(*)[16]>(a));
@@ -533,11 +521,11 @@ inline PFN_cuTensorMapEncodeTiled_v12000 tensor_map_encoder() {
   return fn;
 }
 
-template <int CG, int M, int EPI, bool F16, int MAXP, int RU>
+template <int CG, int M, int EPI, bool F16, int MAXP>
 int launch_g16(const void* x, int64_t x_stride, int64_t x_rows, int slots, const void* w, int experts, int k, int n, const int* items,
                const int* counts, const int* members, void* out, float limit, int64_t max_items, cudaStream_t stream) {
-  using SH = G16Shape<CG, MAXP, RU>;
-  auto* kern = g16_kernel<CG, M, EPI, F16, MAXP, RU>;
+  using SH = G16Shape<CG, MAXP>;
+  auto* kern = g16_kernel<CG, M, EPI, F16, MAXP>;
   static bool configured[64] = {false};
   int dev = 0;
   TFB_CUDA(cudaGetDevice(&dev), "experts16: cudaGetDevice");
@@ -567,7 +555,7 @@ int launch_g16(const void* x, int64_t x_stride, int64_t x_rows, int slots, const
                                 CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     if (wrc != CUDA_SUCCESS) return fail(TFB_ERR_CUDA, "experts16: no tensor map of the weights (%d)", (int)wrc);
   }
-  const int64_t units = max_items * ((w16_rows(M, n) + CG * RU - 1) / (CG * RU));
+  const int64_t units = max_items * ((w16_rows(M, n) + CG * W16_ROWS - 1) / (CG * W16_ROWS));
   if (units >= (int64_t(1) << 30)) return fail(TFB_ERR_ARG, "experts16: too many units");
   const int64_t most = sm_count() / CG, walkers = units < most ? units : most;
   cudaLaunchConfig_t cfg = {};
@@ -587,20 +575,6 @@ int launch_g16(const void* x, int64_t x_stride, int64_t x_rows, int slots, const
   return check_cuda(cudaLaunchKernelEx(&cfg, kern, map, wmap, slots, static_cast<const uint8_t*>(w), k, n, items, counts, members,
                                        out, limit),
                     "experts16");
-}
-
-// Rows a unit takes: 128 unless 64 or 32 leave the busiest CTA a tenth fewer rows.
-inline int g16_unit_rows(int64_t items, int rows) {
-  int best = 128;
-  int64_t most = 0;
-  for (int ru = 128; ru >= 32; ru /= 2) {
-    const int64_t units = items * ((rows + ru - 1) / ru), load = (units + sm_count() - 1) / sm_count() * ru;
-    if (ru == 128 || load * 10 <= most * 9) {
-      best = ru;
-      most = load;
-    }
-  }
-  return best;
 }
 
 }  // namespace tfb
@@ -655,16 +629,14 @@ extern "C" int tfb_experts16(int epi, int fp16, const void* x, int64_t x_stride,
   TFB_REQUIRE(tile >= 1 && tile <= G16_MAXP, "experts16: items of 1..%d pairs, not %d", G16_MAXP, tile);
   if (max_items == 0 || x_rows == 0) return TFB_OK;
   auto st = static_cast<cudaStream_t>(stream);
-#define TFB_G16_AT(CG_, EPI_, M_, F16_, MAXP_, RU_) \
-  return launch_g16<CG_, M_, EPI_, F16_, MAXP_, RU_>(x, x_stride, x_rows, slots, w, experts, k, n, items, counts, members, out, limit, max_items, st)
-#define TFB_G16(EPI_, M_, F16_)                                   \
-  do {                                                            \
-    if (tile > 128) TFB_G16_AT(2, EPI_, M_, F16_, 256, 128);      \
-    if (tile > 32) TFB_G16_AT(2, EPI_, M_, F16_, 128, 128);       \
-    const int ru = g16_unit_rows(max_items, w16_rows(M_, n));     \
-    if (ru == 128) TFB_G16_AT(1, EPI_, M_, F16_, 32, 128);        \
-    if (ru == 64) TFB_G16_AT(1, EPI_, M_, F16_, 32, 64);          \
-    TFB_G16_AT(1, EPI_, M_, F16_, 32, 32);                        \
+#define TFB_G16_AT(CG_, EPI_, M_, F16_, MAXP_)                                                                              \
+  return launch_g16<CG_, M_, EPI_, F16_, MAXP_>(x, x_stride, x_rows, slots, w, experts, k, n, items, counts, members, out,    \
+                                                limit, max_items, st)
+#define TFB_G16(EPI_, M_, F16_)                             \
+  do {                                                      \
+    if (tile > 128) TFB_G16_AT(2, EPI_, M_, F16_, 256);     \
+    if (tile > 32) TFB_G16_AT(2, EPI_, M_, F16_, 128);      \
+    TFB_G16_AT(1, EPI_, M_, F16_, 32);                      \
   } while (0)
 #define TFB_G16_EPI(EPI_, M_)          \
   if (epi == EPI_) {                   \
