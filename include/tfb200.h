@@ -340,6 +340,16 @@ int tfb_experts16(int epi, int fp16, const void* x, int64_t x_stride, int64_t x_
                   int experts, int k, int n, const int32_t* items, const int32_t* counts, const int32_t* members, void* out, float limit,
                   int64_t max_items, int tile, void* stream);
 
+/* A routed block whose routing is the caller's, behind one call: out [rows, dims] (bf16, or fp32 when out_f32) = the sum over
+ * the slots of wts * down(f(up(x))) of the pick's expert; picks outside 0..experts-1 take no part, a row without any is
+ * zeros.  x, up, down, act in bf16 or fp16; members, items, counts: tfb_plan's tables, scratch here (items for max_items
+ * of at most `tile` pairs; left alone when there are 32 pairs or fewer, which need no plan); act [rows * slots, width] and y
+ * [rows * slots, dims] fp32: scratch. */
+int tfb_experts16_block(int fp16, const void* x, int64_t x_stride, int rows, const int32_t* picks, int slots,
+                        const float* wts, const void* up, int swiglu, float limit, const void* down, int experts,
+                        int dims, int width, int32_t* members, int32_t* items, int32_t* counts, int64_t max_items,
+                        int tile, void* act, float* y, void* out, int out_f32, void* stream);
+
 /* ---- low-rank adapters (no reference counterpart) ------------------------------------------------------------------ */
 
 /* out[m] = base[m] + scale[i] * B[i] (A[i] x[m]) with i = ids[m], the base alone where i is outside 0..count-1.  x

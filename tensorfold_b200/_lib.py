@@ -47,6 +47,7 @@ SIGNATURES: dict[str, tuple] = {
     "tfb_pack16": (P, P, P, I, I, I, P),
     "tfb_unpack16": (P, P, P, I, I, I, P),
     "tfb_experts16": (I, I, P, L, L, I, P, I, I, I, P, P, P, P, F, L, I, P),
+    "tfb_experts16_block": (I, P, L, I, P, I, P, P, I, F, P, I, I, I, P, P, P, L, I, P, P, P, I, P),
     "tfb_adapters": (I, P, L, P, P, P, I, I, I, P, I, I, P, P, P, L, P, I, L, P, I, L, P),
     "tfb_exl3_dequant": (P, P, I, I, I, I, P),
     "tfb_exl3_group": (P, P, P, P, P, P, P, I, I, I, I, I, P),

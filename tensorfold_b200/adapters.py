@@ -130,35 +130,44 @@ def route(ids: torch.Tensor, plan: Plan) -> None:
                       plan.items.data_ptr(), plan.counts.data_ptr(), _lib.stream(ids.device))
 
 
-def _span(t: torch.Tensor) -> tuple[int, int]:
-    last = sum((s - 1) * st for s, st in zip(t.shape, t.stride())) if t.numel() else -1
-    return t.data_ptr(), t.data_ptr() + (last + 1) * t.element_size()
+def _end(t: torch.Tensor, m: int) -> int:
+    """The address behind the last of ``m`` rows."""
+
+    return t.data_ptr() + ((m - 1) * t.stride(0) + t.shape[1]) * t.element_size()
 
 
-def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
-    (a0, a1), (b0, b1) = _span(a), _span(b)
-    return a0 < b1 and b0 < a1
+def _overlap(a: torch.Tensor, b: torch.Tensor, m: int) -> bool:
+    return a.data_ptr() < _end(b, m) and b.data_ptr() < _end(a, m)
 
 
-def _rows_of(t: torch.Tensor, name: str, m: int, n: int, device: torch.device) -> None:
-    if t.dim() != 2 or tuple(t.shape) != (m, n) or t.stride(1) != 1 and n > 1 or t.dtype not in ROW_TYPES:
-        raise ValueError(f"{name}: [{m}, {n}] fp32, bf16 or fp16 with unit-stride rows")
-    if m > 1 and t.stride(0) < n:
+def _rows_of(t: torch.Tensor, name: str, m: int, n: int, device: torch.device) -> tuple[int, int]:
+    """The row type and the step between rows of [m, n] ``t``."""
+
+    kind = ROW_TYPES.get(t.dtype)
+    if kind is None or t.shape != (m, n):
+        raise ValueError(f"{name}: [{m}, {n}] fp32, bf16 or fp16, not {t.dtype} {tuple(t.shape)}")
+    row, one = t.stride()
+    if one != 1 and n > 1:
+        raise ValueError(f"{name}: [{m}, {n}] with unit-stride rows")
+    if m > 1 and row < n:
         raise ValueError(f"{name}: rows must not overlap")
     if t.device != device:
         raise ValueError(f"{name} must be on x's device")
+    return kind, row if m > 1 else n
 
 
 def check(x: torch.Tensor, ad: Adapters, plan: Plan) -> None:
     """Refuses what ``add`` cannot take, before a projection in front of it is launched."""
 
-    grouped._need_cuda(x, "x")
-    if x.dim() != 2 or x.dtype != ad.dtype or x.shape[1] != ad.k or x.stride(1) != 1:
+    if not x.is_cuda:
+        raise ValueError("x must be a CUDA tensor (this library has no CPU path)")
+    ids, a = plan.ids, ad.a
+    if x.dim() != 2 or x.dtype != a.dtype or x.shape[1] != ad.k or x.stride(1) != 1:
         raise ValueError(f"x: [M, {ad.k}] {ad.dtype} with unit-stride rows, as the adapters")
-    if ad.device != x.device or plan.members.device != x.device:
-        raise ValueError("x, the adapters and the plan must be on one device")
-    if plan.ids is None or plan.ids.shape[0] != x.shape[0]:
+    if ids is None or ids.shape[0] != x.shape[0]:
         raise ValueError("route(ids, plan) comes first, with one id a row")
+    if a.device != x.device or ids.device != x.device:
+        raise ValueError("x, the adapters and the plan must be on one device")
     if plan.count != ad.count:
         raise ValueError(f"a plan of {plan.count} adapters for {ad.count}")
 
@@ -169,29 +178,38 @@ def add(x: torch.Tensor, ad: Adapters, plan: Plan, base: torch.Tensor, out: torc
     (``dtype``, or ``base``'s, where ``out`` is not given).  ``out`` may be ``base`` itself."""
 
     check(x, ad, plan)
-    m, n = x.shape[0], ad.n
-    _rows_of(base, "base", m, n, x.device)
+    return add_checked(x, ad, plan, base, out, dtype)
+
+
+def add_checked(x: torch.Tensor, ad: Adapters, plan: Plan, base: torch.Tensor, out: torch.Tensor | None,
+                dtype: torch.dtype | None) -> torch.Tensor:
+    """``add`` behind ``check``."""
+
+    m, n, k, device = x.shape[0], ad.n, ad.k, x.device
+    base_type, base_step = _rows_of(base, "base", m, n, device)
     if out is None:
-        out = torch.empty((m, n), dtype=dtype or base.dtype, device=x.device)
-    elif dtype is not None and out.dtype != dtype:
-        raise ValueError(f"out is {out.dtype}, not {dtype}")
-    _rows_of(out, "out", m, n, x.device)
+        out = torch.empty((m, n), dtype=dtype or base.dtype, device=device)
+        out_type, out_step = ROW_TYPES.get(out.dtype), n
+        if out_type is None:
+            raise ValueError(f"out: fp32, bf16 or fp16, not {out.dtype}")
+    else:
+        if dtype is not None and out.dtype != dtype:
+            raise ValueError(f"out is {out.dtype}, not {dtype}")
+        out_type, out_step = _rows_of(out, "out", m, n, device)
+        same = out.data_ptr() == base.data_ptr() and out_type == base_type and out_step == base_step
+        if m and (_overlap(out, x, m) or not same and _overlap(out, base, m)):
+            raise ValueError("out may be base itself, but must not overlap x or a part of base")
     if m == 0:
         return out
-    same = out.data_ptr() == base.data_ptr() and out.dtype == base.dtype and (m == 1 or out.stride(0) == base.stride(0))
-    if _overlap(out, x) or not same and _overlap(out, base):
-        raise ValueError("out may be base itself, but must not overlap x or a part of base")
-    if (x.stride(0) % 8 or x.stride(0) < ad.k) and m > 1 or x.data_ptr() % 16:
-        x = x.clone(memory_format=torch.contiguous_format)          # rows are read in 16-byte pieces
-    def step(t):
-        return t.stride(0) if m > 1 else t.shape[1]
-
-    planned = m > DIRECT_ROWS
-    with _lib.on(x.device):
-        _lib.call("tfb_adapters", int(ad.dtype == torch.float16), x.data_ptr(), step(x), ad.a.data_ptr(), ad.b.data_ptr(),
-                  ad.scale.data_ptr(), ad.a.shape[1], ad.k, n, plan.ids.data_ptr(), m, ad.count,
-                  plan.items.data_ptr() if planned else 0, plan.counts.data_ptr() if planned else 0,
-                  plan.members.data_ptr() if planned else 0, grouped.max_items(m, ad.count, ITEM), base.data_ptr(),
-                  ROW_TYPES[base.dtype], step(base), out.data_ptr(), ROW_TYPES[out.dtype], step(out),
-                  _lib.stream(x.device))
+    x_step = x.stride(0) if m > 1 else k
+    if x_step % 8 or x_step < k or x.data_ptr() % 16:
+        x, x_step = x.clone(memory_format=torch.contiguous_format), k        # rows are read in 16-byte pieces
+    a, items, counts, members, most = ad.a, 0, 0, 0, 0
+    if m > DIRECT_ROWS:
+        items, counts, members = plan.items.data_ptr(), plan.counts.data_ptr(), plan.members.data_ptr()
+        most = grouped.max_items(m, ad.count, ITEM)
+    with _lib.on(device):
+        _lib.call("tfb_adapters", a.dtype == torch.float16, x.data_ptr(), x_step, a.data_ptr(), ad.b.data_ptr(),
+                  ad.scale.data_ptr(), a.shape[1], k, n, plan.ids.data_ptr(), m, ad.count, items, counts, members, most,
+                  base.data_ptr(), base_type, base_step, out.data_ptr(), out_type, out_step, _lib.stream(device))
     return out

@@ -65,6 +65,17 @@ __device__ __forceinline__ void ad_store(void* p, int type, int64_t i, float v) 
   else static_cast<uint16_t*>(p)[i] = type == AD_BF16 ? to16<false>(v) : to16<true>(v);
 }
 
+__device__ __forceinline__ uint2 ldg_nc2(const void* p) {
+  uint2 r;
+  asm volatile("ld.global.nc.v2.u32 {%0, %1}, [%2];\n" : "=r"(r.x), "=r"(r.y) : "l"(p));
+  return r;
+}
+__device__ __forceinline__ uint4 ld_dep_u4(const void* p) {                // base may be out: not the read-only path
+  uint4 r;
+  asm volatile("ld.global.v4.u32 {%0, %1, %2, %3}, [%4];\n" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "l"(p) : "memory");
+  return r;
+}
+
 // the float4 at `p` of this CTA's shared memory, in the same place of CTA `rank` of the cluster
 __device__ __forceinline__ float4 ld_cluster4(const float* p, int rank) {
   uint32_t at;
@@ -74,43 +85,134 @@ __device__ __forceinline__ float4 ld_cluster4(const float* p, int rank) {
   return v;
 }
 
+__device__ __forceinline__ uint32_t cluster_addr(const void* p, int rank) {      // this CTA's `p`, in CTA `rank`
+  uint32_t at;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;\n" : "=r"(at) : "r"(smem_addr(p)), "r"(rank));
+  return at;
+}
+__device__ __forceinline__ void st_cluster2(uint32_t at, uint2 v) {
+  asm volatile("st.shared::cluster.v2.u32 [%0], {%1, %2};\n" ::"r"(at), "r"(v.x), "r"(v.y) : "memory");
+}
+__device__ __forceinline__ void st_cluster1(uint32_t at, float v) {
+  asm volatile("st.shared::cluster.f32 [%0], %1;\n" ::"r"(at), "f"(v) : "memory");
+}
+
+// Eight neighbouring values of a row from column c on, as they are stored (`wide`: 16-byte pieces; else, or at the row's end,
+// one by one), and their way back; ad_widen: what was loaded, in fp32.
+__device__ __forceinline__ bool ad_wide(const void* p, int type, int64_t stride) {
+  return stride % (type == AD_F32 ? 4 : 8) == 0 && (reinterpret_cast<uintptr_t>(p) & 15) == 0;
+}
+__device__ __forceinline__ void ad_load8(const void* p, int type, int64_t at, uint4 (&raw)[2]) {
+  if (type == AD_F32) {
+    raw[0] = ld_dep_u4(static_cast<const float*>(p) + at);
+    raw[1] = ld_dep_u4(static_cast<const float*>(p) + at + 4);
+  } else {
+    raw[0] = ld_dep_u4(static_cast<const uint16_t*>(p) + at);
+  }
+}
+__device__ __forceinline__ void ad_widen(const uint4 (&raw)[2], int type, float (&v)[8]) {
+  const uint32_t w[8] = {raw[0].x, raw[0].y, raw[0].z, raw[0].w, raw[1].x, raw[1].y, raw[1].z, raw[1].w};
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const uint16_t u = (uint16_t)(w[i >> 1] >> (16 * (i & 1)));
+    v[i] = type == AD_F32 ? __uint_as_float(w[i]) : type == AD_BF16 ? from16<false>(u) : from16<true>(u);
+  }
+}
+__device__ __forceinline__ void ad_narrow_load8(const void* p, int type, int64_t at, int have, float (&v)[8]) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v[i] = i < have ? ad_load(p, type, at + i) : 0.f;
+}
+__device__ __forceinline__ void ad_store8(void* p, int type, bool wide, int64_t at, int have, const float (&v)[8]) {
+  if (have < 8 || !wide) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (i < have) ad_store(p, type, at + i, v[i]);
+  } else if (type == AD_F32) {
+    float* o = static_cast<float*>(p) + at;
+    *reinterpret_cast<float4*>(o) = make_float4(v[0], v[1], v[2], v[3]);
+    *reinterpret_cast<float4*>(o + 4) = make_float4(v[4], v[5], v[6], v[7]);
+  } else {
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t a = type == AD_BF16 ? to16<false>(v[2 * i]) : to16<true>(v[2 * i]);
+      const uint32_t b = type == AD_BF16 ? to16<false>(v[2 * i + 1]) : to16<true>(v[2 * i + 1]);
+      w[i] = a | (b << 16);
+    }
+    *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p) + at) = make_uint4(w[0], w[1], w[2], w[3]);
+  }
+}
+
+// Rows r0 .. r0 + B - 1 whose bit is set in `take`, columns 8 `c8` and every `step` eights further: the base alone.
+template <int B>
+__device__ __forceinline__ void ad_copy_rows(const AdArgs& g, int r0, uint32_t take, int c8, int step) {
+  const bool wide_base = ad_wide(g.base, g.base_type, g.base_stride), wide_out = ad_wide(g.out, g.out_type, g.out_stride);
+  for (int c = 8 * c8; c < g.N; c += 8 * step) {
+    const int have = min(8, g.N - c);
+    const bool whole = have == 8 && wide_base;
+    uint4 raw[B][2];
+#pragma unroll
+    for (int i = 0; i < B; ++i)                                            // the rows' loads are in flight together
+      if ((take >> i & 1) && whole) ad_load8(g.base, g.base_type, (r0 + i) * g.base_stride + c, raw[i]);
+#pragma unroll
+    for (int i = 0; i < B; ++i) {
+      if (!(take >> i & 1)) continue;
+      float v[8];
+      if (whole) ad_widen(raw[i], g.base_type, v);
+      else ad_narrow_load8(g.base, g.base_type, (r0 + i) * g.base_stride + c, have, v);
+      ad_store8(g.out, g.out_type, wide_out, (r0 + i) * g.out_stride + c, have, v);
+    }
+  }
+}
+
 // inputs a warp of the cluster takes: K / 32 rounded up to 64
 __host__ __device__ __forceinline__ int ad_run(int k) {
   const int runs = AD_CTAS * AD_WARPS;
   return ((k + runs - 1) / runs + 63) / 64 * 64;
 }
 
+// RT: sixteens of ranks.  NT: eights of rows an item holds; 1 = every row an item of its own (its tile's other rows idle).
 template <int RT, int NT>
-struct AdSmem {
+struct AdShape {
+  static constexpr bool ALONE = NT == 1;
   static constexpr int ROWS = 8 * NT, RP = 16 * RT, PITCH = RP + 4;        // + 4: the partial sums' columns spread over banks
+  static constexpr int MT = (ROWS + 15) / 16;                              // row tiles of the second product
+  static constexpr int QUADS = RP / 4;                                     // fours of a row's ranks
+  static constexpr int SUM_ROWS = ALONE ? 1 : ROWS / AD_CTAS;              // rows a CTA adds up over the cluster
+  static constexpr int KU = NT > 1 ? (RT <= 2 ? 2 : 1) : (RT <= 2 ? 4 : RT == 4 ? 2 : 1);   // steps of 32 inputs loaded at once
+  static constexpr int CH = ALONE && RT <= 2 ? 2 : 1;   // blocks of columns loaded at once
   static constexpr int PART = AD_WARPS * ROWS * PITCH * 4;                 // float part[warp][row][PITCH]; the sum in warp 0's
   static constexpr int LOW = ROWS * RP * 2;                                // hi[row][RP], then lo
   static constexpr int HI_OFFSET = PART;
   static constexpr int BACK_OFFSET = HI_OFFSET + 2 * LOW;                  // float back[row]: the row's scaling undone
   static constexpr int ROW_OFFSET = BACK_OFFSET + ROWS * 4;                // int row[ROWS]
   static constexpr int TOTAL = ROW_OFFSET + ROWS * 4;
+  static_assert(ALONE || ROWS % AD_CTAS == 0, "the cluster shares the rows out");
+  static_assert(SUM_ROWS * QUADS <= AD_WARPS * 32 || SUM_ROWS * QUADS % (AD_WARPS * 32) == 0, "whole warps reduce");
 };
 
 template <int RT, int NT, bool F16>
-__global__ void __launch_bounds__(AD_WARPS * 32)
+__global__ void __launch_bounds__(AD_WARPS * 32, RT == 1 ? 5 : RT == 2 ? 4 : RT == 4 ? 3 : 1)
 adapters_kernel(AdArgs g) {
-  using SM = AdSmem<RT, NT>;
-  constexpr int ROWS = SM::ROWS, RP = SM::RP, PITCH = SM::PITCH;
-  constexpr int MT = (ROWS + 15) / 16;                                     // row tiles of the second product
+  using SH = AdShape<RT, NT>;
+  constexpr int ROWS = SH::ROWS, RP = SH::RP, PITCH = SH::PITCH, MT = SH::MT, QUADS = SH::QUADS, KU = SH::KU, CH = SH::CH;
+  constexpr bool ALONE = SH::ALONE;
+  constexpr int THREADS = AD_WARPS * 32, STRIDE = AD_CTAS * AD_WARPS * 32;   // columns the cluster forms at a time
   extern __shared__ __align__(16) uint8_t ad_smem[];
   float* part = reinterpret_cast<float*>(ad_smem);
-  uint16_t* hi = reinterpret_cast<uint16_t*>(ad_smem + SM::HI_OFFSET);
+  uint16_t* hi = reinterpret_cast<uint16_t*>(ad_smem + SH::HI_OFFSET);
   uint16_t* lo = hi + ROWS * RP;
-  float* back = reinterpret_cast<float*>(ad_smem + SM::BACK_OFFSET);
-  int* row = reinterpret_cast<int*>(ad_smem + SM::ROW_OFFSET);
+  float* back = reinterpret_cast<float*>(ad_smem + SH::BACK_OFFSET);
+  int* row = reinterpret_cast<int*>(ad_smem + SH::ROW_OFFSET);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, gq = lane >> 2, t = lane & 3;
   const int cta = blockIdx.x % AD_CTAS, unit = blockIdx.x / AD_CTAS;
   const int N = g.N, K = g.K, R = g.R;
 
   pdl_wait();
+  pdl_launch_dependents();                                                 // what follows waits for this grid's end all the same
   // ---- which rows, whose adapter (the same for the whole cluster) ----
   int who = -1, first = unit, cnt = 1;
-  if (g.items == nullptr) {
+  if (ALONE) {
     who = ld_dep(g.ids + unit);
     if (who >= g.count) who = -1;
   } else if (unit < g.clusters) {
@@ -122,224 +224,245 @@ adapters_kernel(AdArgs g) {
     cnt = min(ld_dep(g.items + 3 * it + 2) - sub * ROWS, ROWS);
     if (cnt <= 0) return;
   } else {
-    // rows without an adapter, which no item holds: the base alone
-    const int r0 = (unit - g.clusters) * AD_TILE, r1 = min(g.rows, r0 + AD_TILE);
-    for (int r = r0; r < r1; ++r) {
-      const int id = ld_dep(g.ids + r);
-      if (id >= 0 && id < g.count) continue;
-      for (int n = cta * (AD_WARPS * 32) + tid; n < N; n += AD_CTAS * AD_WARPS * 32)
-        ad_store(g.out, g.out_type, r * g.out_stride + n, ad_load(g.base, g.base_type, r * g.base_stride + n));
-    }
+    // rows without an adapter, which no item holds: the base alone; eight rows a CTA, looked at all at once
+    const int r0 = (unit - g.clusters) * AD_TILE + cta * 8, id = r0 + lane < g.rows && lane < 8 ? ld_dep(g.ids + r0 + lane) : 0;
+    const uint32_t take = __ballot_sync(0xffffffffu, id < 0 || id >= g.count);
+#pragma unroll
+    for (int half = 0; half < 8; half += 4)
+      if (take >> half & 15) ad_copy_rows<4>(g, r0 + half, take >> half, tid, THREADS);
     return;
   }
   if (who < 0) {
-    for (int n = cta * (AD_WARPS * 32) + tid; n < N; n += AD_CTAS * AD_WARPS * 32)
-      ad_store(g.out, g.out_type, unit * g.out_stride + n, ad_load(g.base, g.base_type, unit * g.base_stride + n));
+    ad_copy_rows<1>(g, unit, 1, cta * THREADS + tid, AD_CTAS * THREADS);
     return;
   }
-  for (int i = tid; i < ROWS; i += AD_WARPS * 32)
-    row[i] = g.items == nullptr ? unit : ld_dep(g.members + first + min(i, cnt - 1));   // past the last: it again, never stored
+  for (int i = tid; i < ROWS; i += THREADS)
+    row[i] = ALONE ? unit : ld_dep(g.members + first + min(i, cnt - 1));   // past the last: it again, never stored
   __syncthreads();
 
   // ---- the low-rank rows: this warp's run of inputs ----
-  float acc[RT][NT][4];
-#pragma unroll
-  for (int m = 0; m < RT; ++m)
-#pragma unroll
-    for (int n = 0; n < NT; ++n)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) acc[m][n][i] = 0.f;
   {
+    float acc[RT][NT][4];
+#pragma unroll
+    for (int m = 0; m < RT; ++m)
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc[m][n][i] = 0.f;
     const int run = ad_run(K), k0 = (cta * AD_WARPS + warp) * run, k1 = min(K, k0 + run);
     const uint16_t* ap = g.a + ((size_t)who * R + gq) * K + 8 * t;
     const uint16_t* xp[NT];
 #pragma unroll
     for (int n = 0; n < NT; ++n) xp[n] = g.x + (size_t)row[8 * n + gq] * g.x_stride + 8 * t;
     const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
-    for (int k = k0; k < k1; k += 32) {                                    // lane t: inputs k + 8 t .. + 7, in any one order
-      const bool in = k + 8 * t < K;
-      uint4 al[RT], ah[RT], xv[NT];
+    for (int k = k0; k < k1; k += 32 * KU) {                               // lane t: inputs k + 8 t .. + 7, in any one order
+      uint4 al[KU][RT], ah[KU][RT], xv[KU][NT];
 #pragma unroll
-      for (int m = 0; m < RT; ++m) {
-        al[m] = in && 16 * m < R ? ldg_nc(ap + (size_t)(16 * m) * K + k) : zero;
-        ah[m] = in && 16 * m + 8 < R ? ldg_nc(ap + (size_t)(16 * m + 8) * K + k) : zero;
-      }
+      for (int v = 0; v < KU; ++v) {                                       // all of a step's loads are in flight at once
+        const int kv = k + 32 * v;
+        const bool in = kv < k1 && kv + 8 * t < K;
 #pragma unroll
-      for (int n = 0; n < NT; ++n) xv[n] = in && 8 * n < cnt ? ldg_nc(xp[n] + k) : zero;
-#pragma unroll
-      for (int n = 0; n < NT; ++n) {
-        if (8 * n >= cnt) break;
+        for (int n = 0; n < NT; ++n) xv[v][n] = in && 8 * n < cnt ? ldg_nc(xp[n] + kv) : zero;
 #pragma unroll
         for (int m = 0; m < RT; ++m) {
-          mma16<F16>(acc[m][n], al[m].x, ah[m].x, al[m].y, ah[m].y, xv[n].x, xv[n].y);
-          mma16<F16>(acc[m][n], al[m].z, ah[m].z, al[m].w, ah[m].w, xv[n].z, xv[n].w);
+          al[v][m] = in && 16 * m < R ? ldg_nc(ap + (size_t)(16 * m) * K + kv) : zero;
+          ah[v][m] = in && 16 * m + 8 < R ? ldg_nc(ap + (size_t)(16 * m + 8) * K + kv) : zero;
+        }
+      }
+#pragma unroll
+      for (int v = 0; v < KU; ++v) {
+        if (k + 32 * v >= k1) break;
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          if (8 * n >= cnt) break;
+#pragma unroll
+          for (int m = 0; m < RT; ++m) {
+            mma16<F16>(acc[m][n], al[v][m].x, ah[v][m].x, al[v][m].y, ah[v][m].y, xv[v][n].x, xv[v][n].y);
+            mma16<F16>(acc[m][n], al[v][m].z, ah[v][m].z, al[v][m].w, ah[v][m].w, xv[v][n].z, xv[v][n].w);
+          }
         }
       }
     }
+#pragma unroll
+    for (int m = 0; m < RT; ++m)
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        float* p = part + (warp * ROWS + 8 * n + 2 * t) * PITCH + 16 * m + gq;
+        p[0] = acc[m][n][0];
+        p[PITCH] = acc[m][n][1];
+        p[8] = acc[m][n][2];
+        p[PITCH + 8] = acc[m][n][3];
+      }
   }
+
+  // ---- the columns' operands that do not hang on the low-rank rows: on their way before the cluster meets ----
+  // a warp forms 32 columns at a time, lane t columns 8 t .. 8 t + 7 of rows gq and gq + 8 of each tile of 16
+  const uint16_t* bp = g.b + (size_t)who * N * R;
+  uint2 bv[CH][RT][4];
+  auto load_b = [&](int c0) {                                              // lane t: ranks 16 ks + 4 t .. + 3
 #pragma unroll
-  for (int m = 0; m < RT; ++m)
+    for (int c = 0; c < CH; ++c)
 #pragma unroll
-    for (int n = 0; n < NT; ++n) {
-      float* p = part + (warp * ROWS + 8 * n + 2 * t) * PITCH + 16 * m + gq;
-      p[0] = acc[m][n][0];
-      p[PITCH] = acc[m][n][1];
-      p[8] = acc[m][n][2];
-      p[PITCH + 8] = acc[m][n][3];
-    }
+      for (int ks = 0; ks < RT; ++ks)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {                                      // mma column gq of tile j = column 8 (gq / 2) + 2 j + gq % 2
+          const int col = c0 + c * STRIDE + (gq >> 1) * 8 + 2 * j + (gq & 1), r = 16 * ks + 4 * t;
+          bv[c][ks][j] = make_uint2(0u, 0u);
+          if (col < N && r < R) bv[c][ks][j] = ldg_nc2(bp + (size_t)col * R + r);
+        }
+  };
+  const bool wide_base = ad_wide(g.base, g.base_type, g.base_stride), wide_out = ad_wide(g.out, g.out_type, g.out_stride);
+  uint4 pb[CH][MT][2][2];                                                  // the base's values as they are
+  auto load_base = [&](int c0) {
+#pragma unroll
+    for (int c = 0; c < CH; ++c)
+#pragma unroll
+      for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int r = 16 * m + 8 * h + gq, cl = c0 + c * STRIDE + 8 * t;
+          if (r >= cnt || cl + 8 > N || !wide_base) continue;
+          ad_load8(g.base, g.base_type, row[r] * g.base_stride + cl, pb[c][m][h]);
+        }
+  };
+  const int c_first = (cta * AD_WARPS + warp) * 32;
+  load_b(c_first);
+  load_base(c_first);
+
   __syncthreads();
-  for (int i = tid; i < ROWS * RP; i += AD_WARPS * 32) {                   // the CTA's four partial sums, in warp order
-    float* p = part + (i / RP) * PITCH + i % RP;
-    float v = p[0];
+  for (int i = tid; i < (ALONE ? QUADS : ROWS * QUADS); i += THREADS) {    // the CTA's four partial sums, in warp order
+    float4* p = reinterpret_cast<float4*>(part + i / QUADS * PITCH + i % QUADS * 4);
+    float4 v = p[0];
 #pragma unroll
-    for (int w = 1; w < AD_WARPS; ++w) v += p[w * ROWS * PITCH];
+    for (int w = 1; w < AD_WARPS; ++w) {
+      const float4 q = p[w * ROWS * PITCH / 4];
+      v.x += q.x;
+      v.y += q.y;
+      v.z += q.z;
+      v.w += q.w;
+    }
     p[0] = v;
   }
   cluster_arrive();
   cluster_wait();
-  // ---- the cluster's eight, in CTA order, into warp 1's place (nobody reads it from outside); scaled; split in two ----
-  float* sum = part + ROWS * PITCH;
+  // ---- the cluster's eight, in CTA order; scaled; split in two.  Each CTA its share of the rows for all eight (a row alone:
+  // each CTA for itself) ----
   const float scale = g.scale[who];
-  for (int i = tid; i < ROWS * (RP / 4); i += AD_WARPS * 32) {
-    const int at = (i / (RP / 4)) * PITCH + (i % (RP / 4)) * 4;
+  for (int i = tid; i < SH::SUM_ROWS * QUADS; i += THREADS) {
+    const int r = (ALONE ? 0 : cta * SH::SUM_ROWS) + i / QUADS, j = i % QUADS * 4;
     float4 v[AD_CTAS];
 #pragma unroll
-    for (int c = 0; c < AD_CTAS; ++c) v[c] = ld_cluster4(part + at, c);
-    float4 s = v[0];
+    for (int c = 0; c < AD_CTAS; ++c) v[c] = ld_cluster4(part + r * PITCH + j, c);
+    float s[4] = {v[0].x, v[0].y, v[0].z, v[0].w};
 #pragma unroll
     for (int c = 1; c < AD_CTAS; ++c) {
-      s.x += v[c].x;
-      s.y += v[c].y;
-      s.z += v[c].z;
-      s.w += v[c].w;
+      s[0] += v[c].x;
+      s[1] += v[c].y;
+      s[2] += v[c].z;
+      s[3] += v[c].w;
     }
-    sum[at] = s.x * scale;
-    sum[at + 1] = s.y * scale;
-    sum[at + 2] = s.z * scale;
-    sum[at + 3] = s.w * scale;
-  }
-  cluster_arrive();                                                        // this CTA has read its neighbours' sums
-  __syncthreads();
-  for (int r = tid; r < ROWS; r += AD_WARPS * 32) {
     float most = 0.f;
-    for (int j = 0; j < RP; ++j) most = fmaxf(most, fabsf(sum[r * PITCH + j]));
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      s[q] *= scale;
+      most = fmaxf(most, fabsf(s[q]));
+    }
+    constexpr unsigned lanes = SH::SUM_ROWS * QUADS >= 32 ? 0xffffffffu : (1u << (SH::SUM_ROWS * QUADS % 32)) - 1;   // a row's fours are neighbours
+#pragma unroll
+    for (int d = 1; d < QUADS; d *= 2) most = fmaxf(most, __shfl_xor_sync(lanes, most, d));
     int ex = 0;
     if (most > 0.f && most <= 3.0e38f) ex = max(-100, min(100, ilogbf(most)));
     const float down = __uint_as_float((uint32_t)(127 - ex) << 23);        // 2^-ex: exact
-    back[r] = __uint_as_float((uint32_t)(127 + ex) << 23);
-    for (int j = 0; j < RP; ++j) {
-      const float v = sum[r * PITCH + j] * down;
-      const uint16_t h = to16<F16>(v);
-      const float rest = v - from16<F16>(h);
-      hi[r * RP + j] = h;
-      lo[r * RP + j] = to16<F16>(fabsf(rest) < 1.f ? rest : 0.f);          // an infinity or NaN stays in hi alone
+    uint16_t h[4], l[4];
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const float w = s[q] * down;
+      h[q] = to16<F16>(w);
+      const float rest = w - from16<F16>(h[q]);
+      l[q] = to16<F16>(fabsf(rest) < 1.f ? rest : 0.f);                    // an infinity or NaN stays in hi alone
+    }
+    const uint2 hv = make_uint2(h[0] | ((uint32_t)h[1] << 16), h[2] | ((uint32_t)h[3] << 16));
+    const uint2 lv = make_uint2(l[0] | ((uint32_t)l[1] << 16), l[2] | ((uint32_t)l[3] << 16));
+    const float up = __uint_as_float((uint32_t)(127 + ex) << 23);
+    if constexpr (ALONE) {
+      *reinterpret_cast<uint2*>(hi + j) = hv;
+      *reinterpret_cast<uint2*>(lo + j) = lv;
+      if (j == 0) back[0] = up;
+    } else {
+#pragma unroll
+      for (int c = 0; c < AD_CTAS; ++c) {
+        st_cluster2(cluster_addr(hi + r * RP + j, c), hv);
+        st_cluster2(cluster_addr(lo + r * RP + j, c), lv);
+        if (j == 0) st_cluster1(cluster_addr(back + r, c), up);
+      }
     }
   }
-  __syncthreads();
+  cluster_arrive();
+  if constexpr (ALONE) __syncthreads();
+  else cluster_wait();
 
-  // ---- an eighth of the columns, 32 a warp at a time: lane t holds columns 8 t .. 8 t + 7 of rows gq, gq + 8 of each tile ----
-  const bool wide_base = (g.base_type == AD_F32 ? g.base_stride % 4 : g.base_stride % 8) == 0 && (reinterpret_cast<uintptr_t>(g.base) & 15) == 0;
-  const bool wide_out = (g.out_type == AD_F32 ? g.out_stride % 4 : g.out_stride % 8) == 0 && (reinterpret_cast<uintptr_t>(g.out) & 15) == 0;
-  const uint16_t* bp = g.b + (size_t)who * N * R;
-  for (int c0 = (warp * AD_CTAS + cta) * 32; c0 < N; c0 += AD_CTAS * AD_WARPS * 32) {
-    float d[MT][4][4];
+  // ---- an eighth of the columns ----
+  for (int c0 = c_first; c0 < N; c0 += CH * STRIDE) {
 #pragma unroll
-    for (int m = 0; m < MT; ++m)
+    for (int c = 0; c < CH; ++c) {
+      float d[MT][4][4];
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
+      for (int m = 0; m < MT; ++m)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) d[m][j][i] = 0.f;
+        for (int j = 0; j < 4; ++j)
 #pragma unroll
-    for (int ks = 0; ks < RT; ++ks) {                                      // lane t: ranks 16 ks + 4 t .. + 3
-      uint2 bv[4];
+          for (int i = 0; i < 4; ++i) d[m][j][i] = 0.f;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {                                        // mma column gq of tile j = column 8 (gq / 2) + 2 j + gq % 2
-        const int col = c0 + (gq >> 1) * 8 + 2 * j + (gq & 1), r = 16 * ks + 4 * t;
-        bv[j] = col < N && r < R ? __ldg(reinterpret_cast<const uint2*>(bp + (size_t)col * R + r)) : make_uint2(0u, 0u);
-      }
+      for (int ks = 0; ks < RT; ++ks)
 #pragma unroll
-      for (int m = 0; m < MT; ++m) {
-        if (16 * m >= cnt) break;
-        const int ra = (16 * m + gq) * RP + 16 * ks + 4 * t, rb = ROWS > 8 ? ra + 8 * RP : ra;
-        const uint2 ha = *reinterpret_cast<const uint2*>(hi + ra), hb = *reinterpret_cast<const uint2*>(hi + rb);
-        const uint2 la = *reinterpret_cast<const uint2*>(lo + ra), lb = *reinterpret_cast<const uint2*>(lo + rb);
+        for (int m = 0; m < MT; ++m) {
+          if (16 * m >= cnt) break;
+          const int ra = (ALONE ? 0 : 16 * m + gq) * RP + 16 * ks + 4 * t, rb = ALONE ? ra : ra + 8 * RP;
+          const uint2 ha = *reinterpret_cast<const uint2*>(hi + ra), hb = *reinterpret_cast<const uint2*>(hi + rb);
+          const uint2 la = *reinterpret_cast<const uint2*>(lo + ra), lb = *reinterpret_cast<const uint2*>(lo + rb);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          mma16<F16>(d[m][j], la.x, lb.x, la.y, lb.y, bv[j].x, bv[j].y);
-          mma16<F16>(d[m][j], ha.x, hb.x, ha.y, hb.y, bv[j].x, bv[j].y);
+          for (int j = 0; j < 4; ++j) {
+            mma16<F16>(d[m][j], la.x, lb.x, la.y, lb.y, bv[c][ks][j].x, bv[c][ks][j].y);
+            mma16<F16>(d[m][j], ha.x, hb.x, ha.y, hb.y, bv[c][ks][j].x, bv[c][ks][j].y);
+          }
         }
-      }
+      if (c == CH - 1 && c0 + CH * STRIDE < N) load_b(c0 + CH * STRIDE);
+      const int cl = c0 + c * STRIDE + 8 * t;                              // the lane's eight columns
+#pragma unroll
+      for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int r = 16 * m + 8 * h + gq;
+          if (r >= cnt || cl >= N) continue;
+          const float bk = back[r];
+          const int have = min(8, N - cl);
+          float v[8];
+          if (have == 8 && wide_base) ad_widen(pb[c][m][h], g.base_type, v);
+          else ad_narrow_load8(g.base, g.base_type, row[r] * g.base_stride + cl, have, v);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            v[2 * j] = fmaf(d[m][j][2 * h], bk, v[2 * j]);
+            v[2 * j + 1] = fmaf(d[m][j][2 * h + 1], bk, v[2 * j + 1]);
+          }
+          ad_store8(g.out, g.out_type, wide_out, row[r] * g.out_stride + cl, have, v);
+        }
     }
-    const int cl = c0 + 8 * t;                                             // the lane's eight columns
-#pragma unroll
-    for (int m = 0; m < MT; ++m)
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const int r = 16 * m + 8 * h + gq;
-        if (r >= cnt || cl >= N) continue;
-        const float bk = back[r];
-        const int64_t at_b = row[r] * g.base_stride + cl, at_o = row[r] * g.out_stride + cl;
-        float v[8];
-        if (cl + 8 <= N && wide_base) {
-          if (g.base_type == AD_F32) {
-            const float4 p = *reinterpret_cast<const float4*>(static_cast<const float*>(g.base) + at_b);
-            const float4 q = *reinterpret_cast<const float4*>(static_cast<const float*>(g.base) + at_b + 4);
-            v[0] = p.x; v[1] = p.y; v[2] = p.z; v[3] = p.w; v[4] = q.x; v[5] = q.y; v[6] = q.z; v[7] = q.w;
-          } else {
-            const uint4 p = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(g.base) + at_b);
-            const uint32_t w[4] = {p.x, p.y, p.z, p.w};
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              const uint16_t u = (uint16_t)(w[i >> 1] >> (16 * (i & 1)));
-              v[i] = g.base_type == AD_BF16 ? from16<false>(u) : from16<true>(u);
-            }
-          }
-        } else {
-#pragma unroll
-          for (int i = 0; i < 8; ++i) v[i] = cl + i < N ? ad_load(g.base, g.base_type, at_b + i) : 0.f;
-        }
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          v[2 * j] = fmaf(d[m][j][2 * h], bk, v[2 * j]);
-          v[2 * j + 1] = fmaf(d[m][j][2 * h + 1], bk, v[2 * j + 1]);
-        }
-        if (cl + 8 <= N && wide_out) {
-          if (g.out_type == AD_F32) {
-            float* o = static_cast<float*>(g.out) + at_o;
-            *reinterpret_cast<float4*>(o) = make_float4(v[0], v[1], v[2], v[3]);
-            *reinterpret_cast<float4*>(o + 4) = make_float4(v[4], v[5], v[6], v[7]);
-          } else {
-            uint32_t w[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const uint32_t a16 = g.out_type == AD_BF16 ? to16<false>(v[2 * i]) : to16<true>(v[2 * i]);
-              const uint32_t b16 = g.out_type == AD_BF16 ? to16<false>(v[2 * i + 1]) : to16<true>(v[2 * i + 1]);
-              w[i] = a16 | (b16 << 16);
-            }
-            *reinterpret_cast<uint4*>(static_cast<uint16_t*>(g.out) + at_o) = make_uint4(w[0], w[1], w[2], w[3]);
-          }
-        } else {
-#pragma unroll
-          for (int i = 0; i < 8; ++i)
-            if (cl + i < N) ad_store(g.out, g.out_type, at_o + i, v[i]);
-        }
-      }
+    if (c0 + CH * STRIDE < N) load_base(c0 + CH * STRIDE);
   }
-  pdl_launch_dependents();
-  cluster_wait();                                                          // nobody reads this CTA's sums any more
+  if constexpr (ALONE) cluster_wait();                                     // nobody reads this CTA's sums any more
 }
 
 template <int RT, int NT, bool F16>
 int launch_adapters(const AdArgs& g, int64_t units, cudaStream_t stream) {
-  using SM = AdSmem<RT, NT>;
+  using SH = AdShape<RT, NT>;
   auto* kern = adapters_kernel<RT, NT, F16>;
-  if constexpr (SM::TOTAL > 48 * 1024) {
+  if constexpr (SH::TOTAL > 48 * 1024) {
     static bool configured[64] = {false};
     int dev = 0;
     TFB_CUDA(cudaGetDevice(&dev), "adapters: cudaGetDevice");
     if (dev < 0 || dev >= 64) return fail(TFB_ERR_ARG, "adapters: device index %d out of range", dev);
     if (!configured[dev]) {
-      TFB_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, SM::TOTAL),
+      TFB_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, SH::TOTAL),
                "adapters: shared memory opt-in");
       configured[dev] = true;
     }
@@ -347,7 +470,7 @@ int launch_adapters(const AdArgs& g, int64_t units, cudaStream_t stream) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(units * AD_CTAS));
   cfg.blockDim = dim3(AD_WARPS * 32);
-  cfg.dynamicSmemBytes = SM::TOTAL;
+  cfg.dynamicSmemBytes = SH::TOTAL;
   cfg.stream = stream;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -406,9 +529,9 @@ extern "C" int tfb_adapters(int fp16, const void* x, int64_t x_stride, const voi
     if (rank <= 64) TFB_AD(4, 1);
     TFB_AD(8, 1);
   }
-  if (rank <= 16) TFB_AD(1, 8);
-  if (rank <= 32) TFB_AD(2, 8);
-  if (rank <= 64) TFB_AD(4, 8);
+  if (rank <= 16) TFB_AD(1, 4);
+  if (rank <= 32) TFB_AD(2, 4);
+  if (rank <= 64) TFB_AD(4, 4);
   TFB_AD(8, 2);
 #undef TFB_AD
 }

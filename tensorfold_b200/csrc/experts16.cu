@@ -84,6 +84,7 @@ unpack16_kernel(const uint4* packed, uint8_t* m0, uint8_t* m1, int mats, int n, 
 // A role's loop runs in all lanes of its warp with one lane elected for the issue: addresses and descriptors stay in uniform
 // registers.  (In a loop of lane 0 alone an MMA took 80 cycles to issue, and at few pairs that was the kernel's time.)
 constexpr int G16_MAXP = 256;                      // pairs an item may hold (MMA N)
+constexpr int G16_FEW = 32;                        // pairs up to which a launch makes its own plan
 
 template <int CG, int MAXP>
 struct G16Shape {
@@ -95,7 +96,8 @@ struct G16Shape {
   static constexpr int STAGES = (206 * 1024 / STAGE) < 10 ? (206 * 1024 / STAGE) : 10;
   static constexpr int TABLE_OFFSET = STAGES * STAGE;                      // int pair[2][MAXP]
   static constexpr int TURN_OFFSET = TABLE_OFFSET + 2 * MAXP * 4;          // the finishing warps' rows: 2 KB each
-  static constexpr int BAR_OFFSET = TURN_OFFSET + EPI_WARPS * 2048;
+  static constexpr int FEW_OFFSET = TURN_OFFSET + EPI_WARPS * 2048;        // plan_few's items, members and item count
+  static constexpr int BAR_OFFSET = FEW_OFFSET + (4 * G16_FEW + 2) * 4;
   static constexpr int TMEM_OFFSET = BAR_OFFSET + (2 * STAGES + 4) * 8;
   static constexpr int TOTAL = TMEM_OFFSET + 16 + 1024;                    // + slack to align the tiles to 1024 bytes
   static constexpr int ACC_COLS = MAXP;                                    // tensor memory: two accumulators
@@ -238,6 +240,45 @@ __device__ __forceinline__ void tma_rows_pair(void* dst, const CUtensorMap* map,
       : "memory");
 }
 
+__device__ __forceinline__ int ld_any(const int* p) {                      // ld_dep, of a table in global or in shared memory
+  int v;
+  asm volatile("ld.s32 %0, [%1];\n" : "=r"(v) : "l"(p) : "memory");
+  return v;
+}
+
+// The plan of at most 32 pairs, by one warp into shared memory: what tfb_plan writes, without a launch and two reads of
+// global memory in a row (one token of 128 experts: 3.5 us and 1 us).  A lane holds a pair.
+__device__ __forceinline__ void plan_few(const int* picks, int pairs, int experts, int tile, int* items, int* members, int* n_items) {
+  const int lane = threadIdx.x & 31;
+  const int pick = lane < pairs ? ld_dep(picks + lane) : -1;
+  const bool live = pick >= 0 && pick < experts;
+  const int e = live ? pick : 0x7FFFFFFF;
+  int before = 0, same = 0, mine = 0;                // pairs of lower experts; of this one; of this one in lower lanes
+#pragma unroll
+  for (int q = 0; q < 32; ++q) {
+    const int o = __shfl_sync(0xffffffffu, e, q);
+    before += o < e;
+    same += o == e;
+    mine += o == e && q < lane;
+  }
+  const bool head = live && mine % tile == 0;        // opens an item
+  int at = 0;                                        // items of lower experts, or earlier ones of this expert
+#pragma unroll
+  for (int q = 0; q < 32; ++q) {
+    const int o = __shfl_sync(0xffffffffu, e, q);
+    const bool opens = __shfl_sync(0xffffffffu, (int)head, q);
+    at += opens && (o < e || (o == e && q < lane));
+  }
+  if (live) members[before + mine] = lane;
+  if (head) {
+    items[3 * at] = e;
+    items[3 * at + 1] = before + mine;
+    items[3 * at + 2] = min(tile, same - mine);
+  }
+  const unsigned heads = __ballot_sync(0xffffffffu, head);
+  if (lane == 0) *n_items = __popc(heads);
+}
+
 struct RingAt {                                     // a walk around the ring of stages
   int s = 0;
   uint32_t ph = 0;
@@ -269,7 +310,7 @@ struct RingAt {                                     // a walk around the ring of
 template <int CG, int M, int EPI, bool F16, int MAXP>
 __global__ void __launch_bounds__(G16Shape<CG, MAXP>::THREADS, 1)
 g16_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ CUtensorMap wmap, int slots, const uint8_t* __restrict__ W, int K, int N,
-           const int* __restrict__ items, const int* __restrict__ counts, const int* __restrict__ members,
+           const int* items, const int* counts, const int* members, const int* picks, int pairs, int experts, int tile,
            void* __restrict__ out, float limit) {
   using SH = G16Shape<CG, MAXP>;
   constexpr int STAGES = SH::STAGES, B_WARPS = SH::B_WARPS;
@@ -302,7 +343,15 @@ g16_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ CUt
   }
   if (warp == SH::MMA_WARP) g16_alloc<CG>(tmem_slot, 2 * SH::ACC_COLS);
   pdl_wait();
-  after_wait(items, counts, members);
+  pdl_launch_dependents();                          // what follows waits for this grid's end all the same: its start is hidden
+  after_wait(items, counts, members, picks);
+  if (picks != nullptr) {
+    int* few = reinterpret_cast<int*>(smem + SH::FEW_OFFSET);
+    if (warp == 0) plan_few(picks, pairs, experts, tile, few, few + 3 * G16_FEW, few + 4 * G16_FEW);
+    items = few;
+    members = few + 3 * G16_FEW;
+    counts = few + 4 * G16_FEW;
+  }
   tc_fence_before();
   __syncthreads();
   if constexpr (CG == 2) {
@@ -311,21 +360,21 @@ g16_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ CUt
   }
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
-  const int units = __shfl_sync(0xffffffffu, ld_dep(counts), 0) * nct;
+  const int units = __shfl_sync(0xffffffffu, ld_any(counts), 0) * nct;
   bool ok = true;
   auto item = [&](int u) { return min(u, units - 1) / nct; };              // of the next unit, or any where there is none
 
   if (units == 0) {
   } else if (warp == SH::A_WARP) {
     RingAt at;
-    int e = ld_dep(items + 3 * item(u0));
+    int e = ld_any(items + 3 * item(u0));
     for (int u = u0; u < units && ok; u += du) {
       const int r0 = ((u - u / nct * nct) * CG + cta) * W16_ROWS, t0 = r0 < rows ? r0 : 0;   // a second CTA without rows: any
       const int rt = min(W16_ROWS, rows - t0);
       const int ee = __shfl_sync(0xffffffffu, e, 0);
       const uint8_t* src = W + ((size_t)ee * rows + t0) * KB * 128;
       const int row = (ee * rows + t0) * KB;
-      e = ld_dep(items + 3 * item(u + du));
+      e = ld_any(items + 3 * item(u + du));
       for (int f = 0; f < KB; ++f) {
         ok = mbar_wait_warp(empty + at.s, at.ph ^ 1);                      // the ring's first round finds every stage free
         if (!ok) break;
@@ -355,15 +404,15 @@ g16_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ CUt
     int next_cnt;
     auto fetch = [&](int u) {
       const int it = item(u);
-      const int first = ld_dep(items + 3 * it + 1);
-      next_cnt = min(ld_dep(items + 3 * it + 2), MAXP);
+      const int first = ld_any(items + 3 * it + 1);
+      next_cnt = min(ld_any(items + 3 * it + 2), MAXP);
       const int half = (next_cnt + SH::STEP - 1) / SH::STEP * SH::STEP / CG;   // pairs of this CTA
       const int p = cta * half + 4 * g;                                    // rows past the last pair repeat it: never stored
       if (lane < SH::LANES) {
-        next.x = ld_dep(members + first + min(p, next_cnt - 1));
-        next.y = ld_dep(members + first + min(p + 1, next_cnt - 1));
-        next.z = ld_dep(members + first + min(p + 2, next_cnt - 1));
-        next.w = ld_dep(members + first + min(p + 3, next_cnt - 1));
+        next.x = ld_any(members + first + min(p, next_cnt - 1));
+        next.y = ld_any(members + first + min(p + 1, next_cnt - 1));
+        next.z = ld_any(members + first + min(p + 2, next_cnt - 1));
+        next.w = ld_any(members + first + min(p + 3, next_cnt - 1));
       }
     };
     fetch(u0);
@@ -396,10 +445,10 @@ g16_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ CUt
       const uint64_t a0 = umma_desc(smem_addr(smem)), b0 = umma_desc(smem_addr(smem + SH::A_BYTES));
       RingAt at;
       int n = 0;                                                           // the CTA's n-th unit
-      int next_cnt = ld_dep(items + 3 * item(u0) + 2);
+      int next_cnt = ld_any(items + 3 * item(u0) + 2);
       for (int u = u0; u < units && ok; u += du, ++n) {
         const int cnt = min(__shfl_sync(0xffffffffu, next_cnt, 0), MAXP);
-        next_cnt = ld_dep(items + 3 * item(u + du) + 2);
+        next_cnt = ld_any(items + 3 * item(u + du) + 2);
         const uint32_t idesc = g16_idesc<CG, F16>((cnt + SH::STEP - 1) / SH::STEP * SH::STEP);
         const uint32_t acc = tmem_base + (n & 1) * SH::ACC_COLS;
         ok = mbar_wait_warp(acc_free + (n & 1), ((n >> 1) & 1) ^ 1);
@@ -427,13 +476,13 @@ g16_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ CUt
     const int q = warp & 3, part = warp >> 2;                              // quarter of the lanes; share of the pairs
     uint8_t* turn = smem + SH::TURN_OFFSET + warp * 2048;
     int n = 0;
-    int first = ld_dep(items + 3 * item(u0) + 1), cnt = ld_dep(items + 3 * item(u0) + 2);
+    int first = ld_any(items + 3 * item(u0) + 1), cnt = ld_any(items + 3 * item(u0) + 2);
     for (int u = u0; u < units && ok; u += du, ++n) {
       const int r0 = ((u - u / nct * nct) * CG + cta) * W16_ROWS, have = min(cnt, MAXP);
       int* pair = table + (n & 1) * MAXP;
-      for (int i = tid; i < ((have + 31) & ~31); i += SH::EPI_WARPS * 32) pair[i] = i < have ? ld_dep(members + first + i) : -1;
-      first = ld_dep(items + 3 * item(u + du) + 1);
-      cnt = ld_dep(items + 3 * item(u + du) + 2);
+      for (int i = tid; i < ((have + 31) & ~31); i += SH::EPI_WARPS * 32) pair[i] = i < have ? ld_any(members + first + i) : -1;
+      first = ld_any(items + 3 * item(u + du) + 1);
+      cnt = ld_any(items + 3 * item(u + du) + 2);
       asm volatile("bar.sync 1, %0;\n" ::"n"(SH::EPI_WARPS * 32) : "memory");
       ok = mbar_wait_warp(acc_full + (n & 1), (n >> 1) & 1);
       if (!ok) break;
@@ -498,7 +547,6 @@ g16_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ CUt
       }
     }
   }
-  pdl_launch_dependents();
   tc_fence_before();
   __syncthreads();
   if constexpr (CG == 2) {                                                 // nobody arrives on this CTA's barriers any more
@@ -523,7 +571,8 @@ inline PFN_cuTensorMapEncodeTiled_v12000 tensor_map_encoder() {
 
 template <int CG, int M, int EPI, bool F16, int MAXP>
 int launch_g16(const void* x, int64_t x_stride, int64_t x_rows, int slots, const void* w, int experts, int k, int n, const int* items,
-               const int* counts, const int* members, void* out, float limit, int64_t max_items, cudaStream_t stream) {
+               const int* counts, const int* members, const int* picks, int pairs, int tile, void* out, float limit,
+               int64_t max_items, cudaStream_t stream) {
   using SH = G16Shape<CG, MAXP>;
   auto* kern = g16_kernel<CG, M, EPI, F16, MAXP>;
   static bool configured[64] = {false};
@@ -573,7 +622,7 @@ int launch_g16(const void* x, int64_t x_stride, int64_t x_rows, int slots, const
   cfg.attrs = CG == 1 ? attr + 1 : attr;
   cfg.numAttrs = (CG == 1 ? 0 : 1) + (g_use_pdl ? 1 : 0);
   return check_cuda(cudaLaunchKernelEx(&cfg, kern, map, wmap, slots, static_cast<const uint8_t*>(w), k, n, items, counts, members,
-                                       out, limit),
+                                       picks, pairs, experts, tile, out, limit),
                     "experts16");
 }
 
@@ -612,26 +661,13 @@ extern "C" int tfb_unpack16(const void* packed, void* m0, void* m1, int experts,
                     "unpack16");
 }
 
-// The grouped product of 16-bit experts over a plan.  epi: 0 fp32 out, 1 relu^2, 2 SwiGLU over (gate, up), 3 rounded to the
-// weights' type; 1 and 2 round to it too.  x: [x_rows, k] rows `x_stride` elements apart; pair p reads row p / slots, or p
-// when slots is 0.  out: [P, n], row p of pair p.  max_items: an upper bound of the plan's items, which hold at most `tile`
-// pairs (1..256).
-extern "C" int tfb_experts16(int epi, int fp16, const void* x, int64_t x_stride, int64_t x_rows, int slots, const void* w,
-                             int experts, int k, int n, const int32_t* items, const int32_t* counts, const int32_t* members, void* out,
-                             float limit, int64_t max_items, int tile, void* stream) {
-  TFB_REQUIRE(x && w && items && counts && members && out, "experts16: null pointer");
-  TFB_REQUIRE(k >= 8 && k % 8 == 0 && k < (1 << 24) && n >= 1 && n < (1 << 24),
-              "experts16: %d columns of %d inputs (inputs in multiples of 8)", n, k);
-  TFB_REQUIRE(aligned16(x) && x_stride % 8 == 0 && x_stride >= k && x_rows >= 0 && x_rows < (int64_t(1) << 31),
-              "experts16: x rows of K inputs, 16-byte aligned");
-  TFB_REQUIRE(aligned16(w), "experts16: w must be 16-byte aligned");
-  TFB_REQUIRE(slots >= 0 && max_items >= 0 && experts >= 1, "experts16: bad slots, item or expert count");
-  TFB_REQUIRE(tile >= 1 && tile <= G16_MAXP, "experts16: items of 1..%d pairs, not %d", G16_MAXP, tile);
-  if (max_items == 0 || x_rows == 0) return TFB_OK;
-  auto st = static_cast<cudaStream_t>(stream);
+// `picks` null: over the plan in items, counts and members; else these are not read and the launch sorts the `pairs` picks.
+static int experts16_run(int epi, int fp16, const void* x, int64_t x_stride, int64_t x_rows, int slots, const void* w, int experts,
+                         int k, int n, const int32_t* items, const int32_t* counts, const int32_t* members, const int32_t* picks,
+                         int pairs, void* out, float limit, int64_t max_items, int tile, cudaStream_t st) {
 #define TFB_G16_AT(CG_, EPI_, M_, F16_, MAXP_)                                                                              \
-  return launch_g16<CG_, M_, EPI_, F16_, MAXP_>(x, x_stride, x_rows, slots, w, experts, k, n, items, counts, members, out,    \
-                                                limit, max_items, st)
+  return launch_g16<CG_, M_, EPI_, F16_, MAXP_>(x, x_stride, x_rows, slots, w, experts, k, n, items, counts, members, picks,  \
+                                                pairs, tile, out, limit, max_items, st)
 #define TFB_G16(EPI_, M_, F16_)                             \
   do {                                                      \
     if (tile > 128) TFB_G16_AT(2, EPI_, M_, F16_, 256);     \
@@ -648,4 +684,55 @@ extern "C" int tfb_experts16(int epi, int fp16, const void* x, int64_t x_stride,
 #undef TFB_G16_AT
 #undef TFB_G16_EPI
   return fail(TFB_ERR_ARG, "experts16: no kernel for epilogue %d", epi);
+}
+
+static int experts16_check(const void* x, int64_t x_stride, int64_t x_rows, const void* w, int experts, int k, int n, int tile) {
+  TFB_REQUIRE(k >= 8 && k % 8 == 0 && k < (1 << 24) && n >= 1 && n < (1 << 24),
+              "experts16: %d columns of %d inputs (inputs in multiples of 8)", n, k);
+  TFB_REQUIRE(aligned16(x) && x_stride % 8 == 0 && x_stride >= k && x_rows >= 0 && x_rows < (int64_t(1) << 31),
+              "experts16: x rows of K inputs, 16-byte aligned");
+  TFB_REQUIRE(aligned16(w), "experts16: w must be 16-byte aligned");
+  TFB_REQUIRE(experts >= 1, "experts16: bad expert count");
+  TFB_REQUIRE(tile >= 1 && tile <= G16_MAXP, "experts16: items of 1..%d pairs, not %d", G16_MAXP, tile);
+  return TFB_OK;
+}
+
+// The grouped product of 16-bit experts over a plan.  epi: 0 fp32 out, 1 relu^2, 2 SwiGLU over (gate, up), 3 rounded to the
+// weights' type; 1 and 2 round to it too.  x: [x_rows, k] rows `x_stride` elements apart; pair p reads row p / slots, or p
+// when slots is 0.  out: [P, n], row p of pair p.  max_items: an upper bound of the plan's items, which hold at most `tile`
+// pairs (1..256).
+extern "C" int tfb_experts16(int epi, int fp16, const void* x, int64_t x_stride, int64_t x_rows, int slots, const void* w,
+                             int experts, int k, int n, const int32_t* items, const int32_t* counts, const int32_t* members,
+                             void* out, float limit, int64_t max_items, int tile, void* stream) {
+  TFB_REQUIRE(x && w && items && counts && members && out, "experts16: null pointer");
+  if (int rc = experts16_check(x, x_stride, x_rows, w, experts, k, n, tile)) return rc;
+  TFB_REQUIRE(slots >= 0 && max_items >= 0, "experts16: bad slots or item count");
+  TFB_REQUIRE(epi >= EPI_F32 && epi <= EPI_BF16, "experts16: no kernel for epilogue %d", epi);
+  if (max_items == 0 || x_rows == 0) return TFB_OK;
+  return experts16_run(epi, fp16, x, x_stride, x_rows, slots, w, experts, k, n, items, counts, members, nullptr, 0, out, limit,
+                       max_items, tile, static_cast<cudaStream_t>(stream));
+}
+
+// The whole routed block behind one call: plan, gate/up, down and the weighted sum over the slots whose pick names an expert.
+extern "C" int tfb_experts16_block(int fp16, const void* x, int64_t x_stride, int rows, const int32_t* picks, int slots,
+                                   const float* wts, const void* up, int swiglu, float limit, const void* down, int experts,
+                                   int dims, int width, int32_t* members, int32_t* items, int32_t* counts, int64_t max_items,
+                                   int tile, void* act, float* y, void* out, int out_f32, void* stream) {
+  TFB_REQUIRE(x && picks && wts && up && down && members && items && counts && act && y && out, "experts16: null pointer");
+  if (int rc = experts16_check(x, x_stride, rows, up, experts, dims, width, tile)) return rc;
+  TFB_REQUIRE(slots >= 1 && (int64_t)rows * slots < (int64_t(1) << 30) && max_items >= 0, "experts16: bad slots or item count");
+  if (int rc = experts16_check(act, width, (int64_t)rows * slots, down, experts, width, dims, tile)) return rc;
+  if (rows == 0) return TFB_OK;
+  auto st = static_cast<cudaStream_t>(stream);
+  const int pairs = rows * slots;
+  const int32_t* few = pairs <= G16_FEW ? picks : nullptr;
+  if (few == nullptr)
+    if (int rc = tfb_plan(picks, pairs, experts, tile, members, items, counts, stream)) return rc;
+  if (int rc = experts16_run(swiglu ? EPI_SWIGLU : EPI_RELU2, fp16, x, x_stride, rows, slots, up, experts, dims, width, items,
+                             counts, members, few, pairs, act, limit, max_items, tile, st))
+    return rc;
+  if (int rc = experts16_run(EPI_F32, fp16, act, width, pairs, 0, down, experts, width, dims, items, counts, members, few, pairs,
+                             y, 0.f, max_items, tile, st))
+    return rc;
+  return tfb_combine_window(y, 0, wts, picks, 0, experts, out, out_f32, rows, slots, dims, stream);
 }

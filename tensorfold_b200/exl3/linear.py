@@ -144,8 +144,8 @@ class Exl3Linear:
         want = out_dtype or (out.dtype if out is not None else x.dtype)
         if adapters is not None:
             if out is None and want in low_rank.ROW_TYPES:
-                return low_rank.add(x, adapters, plan, y, dtype=want)
-            low_rank.add(x, adapters, plan, y, y)
+                return low_rank.add_checked(x, adapters, plan, y, None, want)
+            low_rank.add_checked(x, adapters, plan, y, y, None)
         if out is None:
             return y.to(want)
         out.copy_(y)

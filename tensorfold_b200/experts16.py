@@ -125,15 +125,18 @@ class Plan(grouped.Plan):
 def _run(epi: int, x: torch.Tensor, slots: int, w: torch.Tensor, k: int, n: int, plan: grouped.Plan, out: torch.Tensor,
          limit: float, rows: int) -> None:
     grouped._need_cuda(x, "x")
-    pairs = rows * plan.slots
+    pairs, device, dtype = rows * plan.slots, x.device, w.dtype
     need = rows if slots else pairs
-    if x.dtype != w.dtype or x.dim() != 2 or x.shape[1] != k or x.shape[0] < need or x.stride(1) != 1 \
-            or (x.stride(0) % 8 or x.stride(0) < k) and x.shape[0] > 1 or x.data_ptr() % 16:
-        raise ValueError(f"x: at least {need} rows of {k} inputs in the experts' type, 16-byte aligned")
-    want = torch.float32 if epi == 0 else w.dtype
+    shape = x.shape
+    if x.dtype != dtype or len(shape) != 2 or shape[1] != k or shape[0] < need:
+        raise ValueError(f"x: at least {need} rows of {k} inputs in the experts' type, not {x.dtype} {tuple(shape)}")
+    step, one = x.stride()
+    if one != 1 or (step % 8 or step < k) and shape[0] > 1 or x.data_ptr() % 16:
+        raise ValueError(f"x: at least {need} rows of {k} inputs, unit-stride and 16-byte aligned")
+    want = torch.float32 if epi == 0 else dtype
     if out.dtype != want or not out.is_contiguous() or out.dim() < 1 or out.shape[-1] != n or out.numel() < pairs * n:
         raise ValueError(f"out: contiguous {want} rows of {n} columns, one a pair")
-    if out.device != x.device or w.device != x.device or plan.members.device != x.device:
+    if out.device != device or w.device != device or plan.members.device != device:
         raise ValueError("x, the experts, the plan and out must be on one device")
     if not w.is_contiguous():
         raise ValueError("w must be contiguous")
@@ -141,11 +144,10 @@ def _run(epi: int, x: torch.Tensor, slots: int, w: torch.Tensor, k: int, n: int,
         raise ValueError(f"a plan with items of {grouped.TILE} to {ITEM} pairs (experts16.Plan)")
     if rows < 0 or rows > plan.rows:
         raise ValueError(f"{rows} rows do not fit a plan of {plan.rows}")
-    with _lib.on(x.device):
-        _lib.call("tfb_experts16", epi, int(w.dtype == torch.float16), x.data_ptr(), x.stride(0) if x.shape[0] > 1 else k,
-                  need, slots, w.data_ptr(), w.shape[0], k, n, plan.items.data_ptr(), plan.counts.data_ptr(), plan.members.data_ptr(),
-                  out.data_ptr(), float(limit), grouped.max_items(pairs, plan.experts, plan.tile), plan.tile,
-                  _lib.stream(x.device))
+    with _lib.on(device):
+        _lib.call("tfb_experts16", epi, dtype == torch.float16, x.data_ptr(), step if shape[0] > 1 else k, need, slots,
+                  w.data_ptr(), w.shape[0], k, n, plan.items.data_ptr(), plan.counts.data_ptr(), plan.members.data_ptr(),
+                  out.data_ptr(), limit, grouped.max_items(pairs, plan.experts, plan.tile), plan.tile, _lib.stream(device))
 
 
 def _fits(ex: Experts16, plan: grouped.Plan) -> None:

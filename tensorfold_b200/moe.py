@@ -53,7 +53,7 @@ def router(x: torch.Tensor, rows: torch.Tensor, out: torch.Tensor | None = None,
 class MoEBuffers:
     """Static scratch for up to ``rows`` rows (CUDA-graph safe); ``prefill`` picks the experts' prefill arithmetic.
     ``dtype``: the weights' type of 16-bit experts, which have one arithmetic; ``prefill`` then picks the router's form
-    and, for bf16, rows of the down projection that are rounded before the sum over the slots."""
+    alone, and the rows of the down projection stay fp32 up to the sum over the slots."""
 
     def __init__(self, rows: int, cfg, device: torch.device | str, *, prefill: bool = False,
                  shared: bool = True, dtype: torch.dtype | None = None) -> None:
@@ -69,7 +69,7 @@ class MoEBuffers:
             self.plan = experts16.Plan(rows, slots, cfg.num_experts + extra, device)
         self.act = torch.empty((rows, slots, cfg.moe_intermediate_size), dtype=dtype or torch.bfloat16, device=device)
         self.y = torch.empty((rows, slots, cfg.hidden_size), device=device,
-                             dtype=torch.bfloat16 if prefill and dtype != torch.float16 else torch.float32)
+                             dtype=torch.bfloat16 if prefill and dtype is None else torch.float32)
         # arrival counters of the kernels that finish their work in whichever block comes last (zero between calls):
         # the one-launch routing (one a group of eight rows, plus one) and the combine folded into the down projection
         self.arrive_route = torch.zeros((2 + rows // 8,), dtype=torch.int32, device=device)
@@ -319,31 +319,48 @@ def picked(x: torch.Tensor, ex, picks: torch.Tensor, wts: torch.Tensor, *, buf: 
     takes no part, whatever its weight; a row without any comes out as zeros.  The result is bf16, or fp32 when ``out`` is
     (always, for fp16 experts).  ``buf`` (``buffers``) is scratch a program keeps; without it the call allocates its own."""
 
-    rows, slots = picks.shape if picks.dim() == 2 else (-1, -1)
-    if picks.dim() != 2 or x.dim() != 2 or x.shape[0] != rows or x.shape[1] != ex.dims or slots < 1:
+    if x.dim() != 2 or picks.dim() != 2 or x.shape[0] != picks.shape[0] or x.shape[1] != ex.dims or picks.shape[1] < 1:
         raise ValueError(f"picked: x [R, {ex.dims}] and picks [R, slots], not {tuple(x.shape)} and {tuple(picks.shape)}")
-    if not x.is_cuda or picks.device != x.device or wts.device != x.device:
-        raise ValueError("picked: x, picks and wts must be on one CUDA device (this library has no CPU path)")
+    rows, slots = picks.shape
+    device = x.device
+    if not x.is_cuda or picks.device != device or wts.device != device or ex.up.device != device:
+        raise ValueError("picked: x, picks, wts and the experts must be on one CUDA device (this library has no CPU path)")
+    if picks.dtype != torch.int32 or not picks.is_contiguous():
+        raise ValueError("picked: picks must be contiguous int32")
     if wts.dtype != torch.float32 or wts.shape != picks.shape or not wts.is_contiguous():
         raise ValueError(f"picked: wts must be contiguous fp32 {tuple(picks.shape)}")
     if buf is None:
-        buf = buffers(ex, max(rows, 1), slots, prefill=False)
-    if buf.slots != slots or rows > buf.rows or buf.plan.experts != ex.count or buf.act.shape[2] != ex.width \
-            or buf.y.shape[2] != ex.dims:
+        buf = buffers(ex, max(rows, 1), slots)
+    plan, dtype = buf.plan, _weights_type(ex)
+    if buf.slots != slots or rows > buf.rows or plan.experts != ex.count or buf.act.shape[2] != ex.width \
+            or buf.y.shape[2] != ex.dims or buf.act.device != device or buf.act.dtype != (dtype or torch.bfloat16) \
+            or isinstance(plan, experts16.Plan) != (dtype is not None):
         raise ValueError(f"picked: {rows} rows of {slots} do not fit buffers of {buf.rows} x {buf.slots}")
-    half = _weights_type(ex) == torch.float16
+    half = dtype == torch.float16
     if out is None:
-        out = torch.empty((rows, ex.dims), dtype=torch.float32 if half else torch.bfloat16, device=x.device)
-    elif tuple(out.shape) != (rows, ex.dims) or not out.is_contiguous() or out.device != x.device \
+        out = torch.empty((rows, ex.dims), dtype=torch.float32 if half else torch.bfloat16, device=device)
+    elif out.shape != x.shape or not out.is_contiguous() or out.device != device \
             or out.dtype not in ((torch.float32,) if half else (torch.bfloat16, torch.float32)):
         raise ValueError(f"picked: out must be contiguous [{rows}, {ex.dims}] bf16 or fp32 (fp32 for fp16 experts)")
     if rows == 0:
         return out
-    ops = _ops(ex)
-    grouped.route(picks, buf.plan, grouped.prompt_tile(rows * slots, ex.count))
-    ops.gate_up(x, ex, buf.plan, buf.act.view(-1, ex.width), rows)
-    ops.down(buf.act.view(-1, ex.width), ex, buf.plan, buf.y.view(-1, ex.dims), rows)
-    with _lib.on(x.device):
+    if dtype is not None:
+        if x.dtype != dtype:
+            raise ValueError(f"picked: x must be {dtype}, as the experts")
+        step = x.stride()
+        if step[1] != 1 or rows > 1 and (step[0] % 8 or step[0] < ex.dims) or x.data_ptr() % 16:
+            x, step = x.clone(memory_format=torch.contiguous_format), (ex.dims, 1)   # rows are read in 16-byte pieces
+        with _lib.on(device):
+            _lib.call("tfb_experts16_block", half, x.data_ptr(), step[0] if rows > 1 else ex.dims, rows, picks.data_ptr(),
+                      slots, wts.data_ptr(), ex.up.data_ptr(), ex.swiglu, ex.limit, ex.down.data_ptr(), ex.count, ex.dims,
+                      ex.width, plan.members.data_ptr(), plan.items.data_ptr(), plan.counts.data_ptr(),
+                      grouped.max_items(rows * slots, ex.count, plan.decode_tile), plan.decode_tile, buf.act.data_ptr(),
+                      buf.y.data_ptr(), out.data_ptr(), out.dtype == torch.float32, _lib.stream(device))
+        return out
+    grouped.route(picks, plan, grouped.prompt_tile(rows * slots, ex.count))
+    grouped.gate_up(x, ex, plan, buf.act.view(-1, ex.width), rows)
+    grouped.down(buf.act.view(-1, ex.width), ex, plan, buf.y.view(-1, ex.dims), rows)
+    with _lib.on(device):
         _lib.call("tfb_combine_window", buf.y.data_ptr(), 1 if buf.y.dtype == torch.bfloat16 else 0, wts.data_ptr(),
                   picks.data_ptr(), 0, ex.count, out.data_ptr(), 1 if out.dtype == torch.float32 else 0, rows, slots, ex.dims,
                   _stream(x))

@@ -146,7 +146,7 @@ def _adapted(x: torch.Tensor, q: Q4, f32: bool, out: torch.Tensor | None, prefil
     want = torch.float32 if f32 else torch.bfloat16
     if out is not None and (out.shape != (x.shape[0], q.n) or out.dtype != want or not out.is_contiguous()):
         raise ValueError(f"out must be contiguous ({x.shape[0]}, {q.n}) {want}")
-    return low_rank.add(x, adapters, plan, _run(x, q, True, None, prefill), out, dtype=want)
+    return low_rank.add_checked(x, adapters, plan, _run(x, q, True, None, prefill), out, want)
 
 
 def matmul(x: torch.Tensor, q: Q4, xs: torch.Tensor | None = None, *, sk: int | None = None, f32: bool = False,

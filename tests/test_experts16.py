@@ -24,6 +24,12 @@ def test_entry_points_refuse_bad_arguments_before_any_launch():
         bad = list(g16)
         bad[at] = value
         cases.append(("tfb_experts16", tuple(bad), why))
+    block = [0, 16, 64, 4, 16, 2, 16, 16, 1, 0.0, 16, 3, 64, 32, 16, 16, 16, 4, 64, 16, 16, 16, 0, 0]
+    for at, value, why in ((1, 0, "null pointer"), (4, 0, "null pointer"), (20, 0, "null pointer"), (2, 60, "x rows"), (5, 0, "bad slots"),
+                           (12, 60, "multiples of 8"), (13, 36, "multiples of 8"), (18, 300, "items of 1..256"), (11, 0, "expert count")):
+        bad = list(block)
+        bad[at] = value
+        cases.append(("tfb_experts16_block", tuple(bad), why))
     ad = [0, 16, 64, 16, 16, 16, 16, 64, 32, 16, 4, 2, 0, 0, 0, 0, 16, 0, 32, 32, 1, 32, 0]
     for at, value, why in ((1, 0, "null pointer"), (9, 0, "null pointer"), (12, 16, "a whole plan or none"),
                            (6, 12, "ranks up to 128"), (6, 136, "ranks up to 128"), (7, 60, "multiples of 8"),
@@ -42,6 +48,7 @@ def test_calls_without_work_launch_nothing():
 
     _lib.call("tfb_experts16", 0, 0, 16, 64, 0, 2, 16, 3, 64, 32, 16, 16, 16, 16, 0.0, 4, 64, 0)
     _lib.call("tfb_experts16", 0, 0, 16, 64, 8, 2, 16, 3, 64, 32, 16, 16, 16, 16, 0.0, 0, 64, 0)
+    _lib.call("tfb_experts16_block", 0, 16, 64, 0, 16, 2, 16, 16, 1, 0.0, 16, 3, 64, 32, 16, 16, 16, 4, 64, 16, 16, 16, 0, 0)
     _lib.call("tfb_adapters", 0, 16, 64, 16, 16, 16, 16, 64, 32, 16, 0, 2, 0, 0, 0, 0, 16, 0, 32, 32, 1, 32, 0)
 
 

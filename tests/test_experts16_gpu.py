@@ -266,6 +266,29 @@ def test_slots_that_take_no_part(dtype):
     assert (got[7] == 0).all() and (got[19] == 0).all()
 
 
+@pytest.mark.parametrize("rows,slots,count", [(1, 1, 1), (1, 8, 9), (4, 8, 128), (32, 1, 3), (3, 7, 5), (2, 16, 70), (1, 32, 2),
+                                              (31, 1, 1), (11, 3, 64)])
+def test_few_pairs_need_no_plan(rows, slots, count):
+    """Up to 32 pairs the launches sort the picks themselves, repeated and absent ones among them: the bits of the same
+    rows in a call of more pairs, which plans; the plan's tables are left alone."""
+
+    from tensorfold_b200 import experts16, moe
+
+    case = (BF, True, 0.0, count, 136, 72, slots, rows)
+    ex = experts16.make(*weights(case, 73))
+    g = torch.Generator().manual_seed(rows * slots)
+    picks = torch.randint(-1, count + 1, (rows, slots), generator=g).to(torch.int32).to(DEV)
+    x, wts = normal(3, rows, 136), torch.rand((rows, slots), generator=gen(4), device=DEV)
+    many = 33 // (rows * slots) + 1
+    want = moe.picked(x.repeat(many, 1), ex, picks.repeat(many, 1), wts.repeat(many, 1))
+    buf = moe.buffers(ex, rows, slots)
+    for t in (buf.plan.items, buf.plan.members, buf.plan.counts):
+        t.fill_(-9)
+    got = moe.picked(x, ex, picks, wts, buf=buf)
+    assert rows * slots > 32 or all((t == -9).all() for t in (buf.plan.items, buf.plan.members, buf.plan.counts))
+    assert torch.equal(got, want[:rows]) and torch.equal(want[-rows:], want[:rows])
+
+
 def test_a_plan_without_pairs_and_calls_without_rows():
     from tensorfold_b200 import experts16, moe
 
