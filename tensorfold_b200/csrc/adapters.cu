@@ -97,30 +97,43 @@ __device__ __forceinline__ void st_cluster1(uint32_t at, float v) {
   asm volatile("st.shared::cluster.f32 [%0], %1;\n" ::"r"(at), "f"(v) : "memory");
 }
 
-// Eight neighbouring values of a row from column c on, as they are stored (`wide`: 16-byte pieces; else, or at the row's end,
-// one by one), and their way back; ad_widen: what was loaded, in fp32.
+// Eight neighbouring values of a row, loaded as they are stored: in 16-byte pieces when `whole`, else the first `have` one by
+// one (rows that do not start on 16 bytes, a row's end), each in a word of its own; in fp32; and their way back.
 __device__ __forceinline__ bool ad_wide(const void* p, int type, int64_t stride) {
   return stride % (type == AD_F32 ? 4 : 8) == 0 && (reinterpret_cast<uintptr_t>(p) & 15) == 0;
 }
-__device__ __forceinline__ void ad_load8(const void* p, int type, int64_t at, uint4 (&raw)[2]) {
-  if (type == AD_F32) {
-    raw[0] = ld_dep_u4(static_cast<const float*>(p) + at);
-    raw[1] = ld_dep_u4(static_cast<const float*>(p) + at + 4);
-  } else {
-    raw[0] = ld_dep_u4(static_cast<const uint16_t*>(p) + at);
-  }
+__device__ __forceinline__ uint32_t ld_dep_u16(const uint16_t* p) {
+  uint16_t v;
+  asm volatile("ld.global.u16 %0, [%1];\n" : "=h"(v) : "l"(p) : "memory");
+  return v;
 }
-__device__ __forceinline__ void ad_widen(const uint4 (&raw)[2], int type, float (&v)[8]) {
+__device__ __forceinline__ void ad_load8(const void* p, int type, int64_t at, bool whole, int have, uint4 (&raw)[2]) {
+  if (whole) {
+    if (type == AD_F32) {
+      raw[0] = ld_dep_u4(static_cast<const float*>(p) + at);
+      raw[1] = ld_dep_u4(static_cast<const float*>(p) + at + 4);
+    } else {
+      raw[0] = ld_dep_u4(static_cast<const uint16_t*>(p) + at);
+    }
+    return;
+  }
+  uint32_t w[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    w[i] = 0u;
+    if (i < have)
+      w[i] = type == AD_F32 ? (uint32_t)ld_dep(static_cast<const int*>(p) + at + i) : ld_dep_u16(static_cast<const uint16_t*>(p) + at + i);
+  }
+  raw[0] = make_uint4(w[0], w[1], w[2], w[3]);
+  raw[1] = make_uint4(w[4], w[5], w[6], w[7]);
+}
+__device__ __forceinline__ void ad_widen(const uint4 (&raw)[2], int type, bool whole, float (&v)[8]) {
   const uint32_t w[8] = {raw[0].x, raw[0].y, raw[0].z, raw[0].w, raw[1].x, raw[1].y, raw[1].z, raw[1].w};
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    const uint16_t u = (uint16_t)(w[i >> 1] >> (16 * (i & 1)));
+    const uint16_t u = (uint16_t)(whole ? w[i >> 1] >> (16 * (i & 1)) : w[i]);
     v[i] = type == AD_F32 ? __uint_as_float(w[i]) : type == AD_BF16 ? from16<false>(u) : from16<true>(u);
   }
-}
-__device__ __forceinline__ void ad_narrow_load8(const void* p, int type, int64_t at, int have, float (&v)[8]) {
-#pragma unroll
-  for (int i = 0; i < 8; ++i) v[i] = i < have ? ad_load(p, type, at + i) : 0.f;
 }
 __device__ __forceinline__ void ad_store8(void* p, int type, bool wide, int64_t at, int have, const float (&v)[8]) {
   if (have < 8 || !wide) {
@@ -153,14 +166,13 @@ __device__ __forceinline__ void ad_copy_rows(const AdArgs& g, int r0, uint32_t t
     uint4 raw[B][2];
 #pragma unroll
     for (int i = 0; i < B; ++i)                                            // the rows' loads are in flight together
-      if ((take >> i & 1) && whole) ad_load8(g.base, g.base_type, (r0 + i) * g.base_stride + c, raw[i]);
+      if (take >> i & 1) ad_load8(g.base, g.base_type, (int64_t)(r0 + i) * g.base_stride + c, whole, have, raw[i]);
 #pragma unroll
     for (int i = 0; i < B; ++i) {
       if (!(take >> i & 1)) continue;
       float v[8];
-      if (whole) ad_widen(raw[i], g.base_type, v);
-      else ad_narrow_load8(g.base, g.base_type, (r0 + i) * g.base_stride + c, have, v);
-      ad_store8(g.out, g.out_type, wide_out, (r0 + i) * g.out_stride + c, have, v);
+      ad_widen(raw[i], g.base_type, whole, v);
+      ad_store8(g.out, g.out_type, wide_out, (int64_t)(r0 + i) * g.out_stride + c, have, v);
     }
   }
 }
@@ -321,8 +333,8 @@ adapters_kernel(AdArgs g) {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           const int r = 16 * m + 8 * h + gq, cl = c0 + c * STRIDE + 8 * t;
-          if (r >= cnt || cl + 8 > N || !wide_base) continue;
-          ad_load8(g.base, g.base_type, row[r] * g.base_stride + cl, pb[c][m][h]);
+          if (r < cnt && cl < N)
+            ad_load8(g.base, g.base_type, row[r] * g.base_stride + cl, wide_base && cl + 8 <= N, N - cl, pb[c][m][h]);
         }
   };
   const int c_first = (cta * AD_WARPS + warp) * 32;
@@ -437,8 +449,7 @@ adapters_kernel(AdArgs g) {
           const float bk = back[r];
           const int have = min(8, N - cl);
           float v[8];
-          if (have == 8 && wide_base) ad_widen(pb[c][m][h], g.base_type, v);
-          else ad_narrow_load8(g.base, g.base_type, row[r] * g.base_stride + cl, have, v);
+          ad_widen(pb[c][m][h], g.base_type, wide_base && have == 8, v);
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             v[2 * j] = fmaf(d[m][j][2 * h], bk, v[2 * j]);
