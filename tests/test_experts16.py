@@ -67,6 +67,17 @@ def test_weights_that_do_not_fit_together_are_refused():
         experts16.pack(w, torch.zeros((2, 8, 24), dtype=BF))
 
 
+def test_the_4_bit_operators_refuse_16_bit_experts():
+    from tensorfold_b200 import experts, experts16
+
+    ex = experts16.Experts16(torch.zeros((2, 16, 64), dtype=BF), torch.zeros((2, 16, 64), dtype=BF), 16, 16, False)
+    plan, x = experts.Plan(4, 1, 2, "cpu"), torch.zeros((4, 16), dtype=BF)
+    for call in (lambda: experts.gate_up(x, ex, plan, x, 4), lambda: experts.down(x, ex, plan, x, 4),
+                 lambda: experts.down_combine(x, ex, plan, x, 4, x, x, x)):
+        with pytest.raises(ValueError, match="run through experts16"):
+            call()
+
+
 def test_item_sizes():
     from tensorfold_b200 import experts16
 

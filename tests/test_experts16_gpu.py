@@ -409,3 +409,34 @@ def test_refusals_on_the_gpu():
                {"buf": moe.buffers(ex, 8, 3)}, {"picks": picks.cpu()}):
         with pytest.raises(ValueError):
             moe.picked(**{"x": x, "ex": ex, "picks": picks, "wts": wts, **kw})
+
+
+@pytest.mark.parametrize("stacked", [True, False])
+@pytest.mark.parametrize("shared", [True, False])
+def test_a_layer_from_a_checkpoint(tmp_path, stacked, shared):
+    """``load.routed16``: the layer built from the file equals the layer built from the tensors, shared expert last."""
+
+    from safetensors.torch import save_file
+    from tensorfold_b200 import experts16, load, moe
+
+    e, d, n = 5, 64, 40
+    gate, up = (normal(i, e + 1, n, d, scale=0.1) for i in (1, 2))
+    down, rows = normal(3, e + 1, d, n, scale=0.1), normal(4, e + 1, d, scale=0.1)
+    tensors = {"l.mlp.gate.weight": rows[:e]}
+    if shared:
+        tensors["l.mlp.shared_expert_gate.weight"] = rows[e:]
+    for proj, m in (("gate_proj", gate), ("up_proj", up), ("down_proj", down)):
+        if stacked:
+            tensors[f"l.mlp.switch_mlp.{proj}.weight"] = m[:e]
+        else:
+            tensors.update({f"l.mlp.experts.{i}.{proj}.weight": m[i] for i in range(e)})
+        if shared:
+            tensors[f"l.mlp.shared_expert.{proj}.weight"] = m[e]
+    save_file({k: v.cpu().contiguous() for k, v in tensors.items()}, str(tmp_path / "model.safetensors"))
+    layer = load.routed16(load.Checkpoint(tmp_path), "l.mlp.", 2, DEV)
+    have = e + 1 if shared else e
+    want = moe.Routed(rows[:have], experts16.make([gate[:have], up[:have]], down[:have]), 2, shared=shared)
+    assert layer.shared == shared and layer.count == e and torch.equal(layer.router, want.router)
+    assert torch.equal(layer.experts.up, want.experts.up) and torch.equal(layer.experts.down, want.experts.down)
+    x = normal(5, 9, d)
+    assert torch.equal(moe.run(x, layer), moe.run(x, want))
