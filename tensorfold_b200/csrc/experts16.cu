@@ -716,6 +716,7 @@ extern "C" int tfb_experts16_block(int fp16, const void* x, int64_t x_stride, in
   TFB_REQUIRE(x && picks && wts && up && down && members && items && counts && act && y && out, "experts16: null pointer");
   if (int rc = experts16_check(x, x_stride, rows, up, experts, dims, width, tile)) return rc;
   TFB_REQUIRE(slots >= 1 && (int64_t)rows * slots < (int64_t(1) << 30) && max_items >= 0, "experts16: bad slots or item count");
+  TFB_REQUIRE(experts <= PLAN_EMAX, "experts16: at most %d experts, not %d", PLAN_EMAX, experts);
   if (int rc = experts16_check(act, width, (int64_t)rows * slots, down, experts, width, dims, tile)) return rc;
   if (rows == 0) return TFB_OK;
   auto st = static_cast<cudaStream_t>(stream);

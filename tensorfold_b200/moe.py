@@ -338,7 +338,7 @@ def picked(x: torch.Tensor, ex, picks: torch.Tensor, wts: torch.Tensor, *, buf: 
         raise ValueError(f"picked: {rows} rows of {slots} do not fit buffers of {buf.rows} x {buf.slots}")
     half = dtype == torch.float16
     if out is None:
-        out = torch.empty((rows, ex.dims), dtype=torch.float32 if half else torch.bfloat16, device=device)
+        out = torch.empty_strided((rows, ex.dims), (ex.dims, 1), dtype=torch.float32 if half else torch.bfloat16, device=device)
     elif out.shape != x.shape or not out.is_contiguous() or out.device != device \
             or out.dtype not in ((torch.float32,) if half else (torch.bfloat16, torch.float32)):
         raise ValueError(f"picked: out must be contiguous [{rows}, {ex.dims}] bf16 or fp32 (fp32 for fp16 experts)")

@@ -26,7 +26,8 @@ def test_entry_points_refuse_bad_arguments_before_any_launch():
         cases.append(("tfb_experts16", tuple(bad), why))
     block = [0, 16, 64, 4, 16, 2, 16, 16, 1, 0.0, 16, 3, 64, 32, 16, 16, 16, 4, 64, 16, 16, 16, 0, 0]
     for at, value, why in ((1, 0, "null pointer"), (4, 0, "null pointer"), (20, 0, "null pointer"), (2, 60, "x rows"), (5, 0, "bad slots"),
-                           (12, 60, "multiples of 8"), (13, 36, "multiples of 8"), (18, 300, "items of 1..256"), (11, 0, "expert count")):
+                           (12, 60, "multiples of 8"), (13, 36, "multiples of 8"), (18, 300, "items of 1..256"), (11, 0, "expert count"),
+                           (11, 1025, "at most 1024 experts")):
         bad = list(block)
         bad[at] = value
         cases.append(("tfb_experts16_block", tuple(bad), why))

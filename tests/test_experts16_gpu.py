@@ -359,6 +359,27 @@ def test_graph_replays_follow_the_picks_on_their_own_scratch():
             assert torch.equal(got, moe.picked(x, ex, picks, wts))
 
 
+def test_two_streams_at_once():
+    """Blocks of different sizes on two streams, launched in turn without waiting, each with its own scratch."""
+
+    from tensorfold_b200 import experts16, moe
+
+    jobs = []
+    for i, (rows, e, d, n, slots) in enumerate([(400, 6, 512, 264, 2), (3, 9, 256, 136, 4)]):
+        ex = experts16.make(*weights((BF, True, 0.0, e, d, n, slots, rows), 101 + i))
+        x, picks, wts = normal(i, rows, d), picks_of(rows, slots, e, i), torch.rand((rows, slots), generator=gen(i), device=DEV)
+        jobs.append((x, ex, picks, wts, moe.buffers(ex, rows, slots), torch.cuda.Stream(), moe.picked(x, ex, picks, wts)))
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(20):
+        for k, (x, ex, picks, wts, buf, stream, _want) in enumerate(jobs):
+            with torch.cuda.stream(stream):
+                got[k].append(moe.picked(x, ex, picks, wts, buf=buf))
+    torch.cuda.synchronize()
+    for k, job in enumerate(jobs):
+        assert all(torch.equal(g, job[-1]) for g in got[k])
+
+
 def test_offsets_past_32_bits():
     """An output of more than 2^32 bytes: its last rows and columns are the right ones."""
 
