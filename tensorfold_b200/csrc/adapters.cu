@@ -8,6 +8,12 @@
 // of the inputs depends on K alone, so a row's bits depend neither on its item nor on the call.
 // The low-rank row is split into two 16-bit parts (s = hi + lo, after an exact power-of-two scaling of the row), which
 // keeps 16 bits of it or more where one rounding would keep 8: the second product costs nothing beside the bytes.
+//
+// What bounds it.  Few rows: latency, the chain id -> inputs and A -> two meetings of the cluster -> columns: one row 4.9 us, 64
+// rows of as many adapters (4096 x 4096, rank 32; 25 MB) 10 us.  Many: latency too, a block of columns a turn - 8192 rows of
+// 4096 x 4096, rank 16, 68 us for 270 MB (DRAM 44 % of its peak, a warp ready in 0.38 of the cycles, 19 warps an SM).  What
+// counts is the number of rows in flight: items of 64 rows (fewer blocks an SM) took 124 us; the base's values through a
+// ring in shared memory 93 to 149 (the more of it, the fewer blocks); the columns in a launch of their own 88.
 
 #include "api.h"
 #include "common.cuh"

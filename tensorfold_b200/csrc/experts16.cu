@@ -4,9 +4,15 @@
 //   down      y[p, n]   = sum_k act[p, k] D[e(p), n, k]
 //
 // over the (row, slot) pairs p that a plan has sorted by expert into items of at most `tile` pairs of one expert.  The
-// WEIGHTS are the MMA's A operand (128 rows of one expert), an item's PAIRS the B operand (N = pairs rounded up to 16),
-// so an expert with three pairs costs an N of 16 and no padded row is ever written.  One fp32 chain over K in order of
+// WEIGHTS are the MMA's A operand (128 rows of one expert), an item's PAIRS the B operand (N = pairs rounded up to 16 or
+// 32), so an expert with three pairs costs an N of 16 and no padded row is ever written.  One fp32 chain over K in order of
 // inputs: a pair's bits do not depend on its item, on the tile or on the call.
+//
+// What bounds it.  Few pairs an expert: HBM - 64 tokens of 128 experts (2048 x 768, top 8), gate/up 119 us for 793 MB, 1.02 of
+// the copy rate; one token 14 us for 50 MB, of which 9 stream and the rest is start, plan and end.  Some hundred pairs: HBM
+// and the tensor pipe in turn - 1999 tokens 145 us, DRAM 73 % of its peak, tensor pipe 40 % busy.  Many: the tensor pipe, 79 %
+// busy at 4096 tokens of 32 experts (160 us, 1290 TFLOP/s), and on long runs the power cap: 8192 tokens of 160 experts
+// (4096 x 1536) run at 877 MHz and 873 TFLOP/s, 0.82 of what the pipe can do at that clock.
 
 #include "api.h"
 #include "common.cuh"

@@ -18,7 +18,10 @@ from . import experts as grouped
 
 DTYPES = (torch.bfloat16, torch.float16)
 ITEM = 256               # pairs an item holds at most: the tensor-core tile's N
-SMALL_ITEMS = ((16, 32), (96, 128))     # up to so many pairs an expert on average: items of so many
+# Up to so many pairs an expert on average: items of so many.  A smaller tile leaves more of the ring to the weights, a larger
+# one reads them once for more pairs.  128 experts of 2048 x 768, top 8, gate/up + down in us with items of 32 / 128 / 256: 200
+# rows 195 / 194 / 198, 400 rows 202 / 196 / 201, 800 rows 229 / 205 / 207; 1400 rows - / 214 / 218, 1999 rows - / 245 / 235.
+SMALL_ITEMS = ((16, 32), (96, 128))
 
 
 def _rows(mats: int, n: int) -> int:
