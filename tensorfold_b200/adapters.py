@@ -5,7 +5,7 @@
 ``Adapters`` holds a projection's adapters in slots; a slot is filled, replaced or emptied in place while others serve.
 ``Plan`` and ``route`` group a batch's rows by adapter once a step, for every projection of the step.  ``add`` is one
 launch (``csrc/adapters.cu``); ``qmm.matmul``, ``qmm.prefill_matmul`` and ``Exl3Linear`` call it behind their product when
-they are given ``adapters=`` and ``plan=``.  Sums are fp32, the low-rank row is kept to 16 bits or more, and a row's bits
+they are given ``adapters=`` and ``plan=``.  Sums are fp32, the low-rank row is kept to 16 bits or more (22 under fp32 rows), and a row's bits
 depend neither on the other rows nor on their number.  No CPU path.
 """
 

@@ -6,8 +6,10 @@
 // A x of its own run of inputs (mma: ranks x rows), the CTAs add the 32 partial sums in warp order through distributed
 // shared memory, and each CTA then forms an eighth of the columns (mma: rows x columns) on top of the base rows.  The cut
 // of the inputs depends on K alone, so a row's bits depend neither on its item nor on the call.
-// The low-rank row is split into two 16-bit parts (s = hi + lo, after an exact power-of-two scaling of the row), which
-// keeps 16 bits of it or more where one rounding would keep 8: the second product costs nothing beside the bytes.
+// The low-rank row is split into 16-bit parts that add up to it (after an exact power-of-two scaling of the row): two, which keep
+// 16 bits of it (bf16) or 22 (fp16) where one rounding would keep 8 or 11, and for bf16 adapters under fp32 rows a third.
+// (With two those rows came out 1.2e-6 off where a computation in 32 bits is 5e-7; with three everywhere a prompt's rows took
+// 5 to 12 % longer.)
 //
 // What bounds it.  Few rows: latency, the chain id -> inputs and A -> two meetings of the cluster -> columns: one row 4.9 us, 64
 // rows of as many adapters (4096 x 4096, rank 32; 25 MB) 10 us.  Many: latency too, a block of columns a turn - 8192 rows of
@@ -200,9 +202,9 @@ struct AdShape {
   static constexpr int KU = NT > 1 ? (RT <= 2 ? 2 : 1) : (RT <= 2 ? 4 : RT == 4 ? 2 : 1);   // steps of 32 inputs loaded at once
   static constexpr int CH = ALONE && RT <= 2 ? 2 : 1;   // blocks of columns loaded at once
   static constexpr int PART = AD_WARPS * ROWS * PITCH * 4;                 // float part[warp][row][PITCH]; the sum in warp 0's
-  static constexpr int LOW = ROWS * RP * 2;                                // hi[row][RP], then lo
-  static constexpr int HI_OFFSET = PART;
-  static constexpr int BACK_OFFSET = HI_OFFSET + 2 * LOW;                  // float back[row]: the row's scaling undone
+  static constexpr int LOW = ROWS * RP * 2;                                // a part of the low-rank rows, [row][RP]
+  static constexpr int LOW_OFFSET = PART;
+  static constexpr int BACK_OFFSET = LOW_OFFSET + 3 * LOW;                 // float back[row]: the row's scaling undone
   static constexpr int ROW_OFFSET = BACK_OFFSET + ROWS * 4;                // int row[ROWS]
   static constexpr int TOTAL = ROW_OFFSET + ROWS * 4;
   static_assert(ALONE || ROWS % AD_CTAS == 0, "the cluster shares the rows out");
@@ -218,8 +220,9 @@ adapters_kernel(AdArgs g) {
   constexpr int THREADS = AD_WARPS * 32, STRIDE = AD_CTAS * AD_WARPS * 32;   // columns the cluster forms at a time
   extern __shared__ __align__(16) uint8_t ad_smem[];
   float* part = reinterpret_cast<float*>(ad_smem);
-  uint16_t* hi = reinterpret_cast<uint16_t*>(ad_smem + SH::HI_OFFSET);
-  uint16_t* lo = hi + ROWS * RP;
+  constexpr int PARTS = F16 ? 2 : 3;                                       // at most
+  const int parts = F16 || g.out_type != AD_F32 ? 2 : 3;
+  uint16_t* low = reinterpret_cast<uint16_t*>(ad_smem + SH::LOW_OFFSET);
   float* back = reinterpret_cast<float*>(ad_smem + SH::BACK_OFFSET);
   int* row = reinterpret_cast<int*>(ad_smem + SH::ROW_OFFSET);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, gq = lane >> 2, t = lane & 3;
@@ -391,27 +394,34 @@ adapters_kernel(AdArgs g) {
     int ex = 0;
     if (most > 0.f && most <= 3.0e38f) ex = max(-100, min(100, ilogbf(most)));
     const float down = __uint_as_float((uint32_t)(127 - ex) << 23);        // 2^-ex: exact
-    uint16_t h[4], l[4];
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      const float w = s[q] * down;
-      h[q] = to16<F16>(w);
-      const float rest = w - from16<F16>(h[q]);
-      l[q] = to16<F16>(fabsf(rest) < 1.f ? rest : 0.f);                    // an infinity or NaN stays in hi alone
-    }
-    const uint2 hv = make_uint2(h[0] | ((uint32_t)h[1] << 16), h[2] | ((uint32_t)h[3] << 16));
-    const uint2 lv = make_uint2(l[0] | ((uint32_t)l[1] << 16), l[2] | ((uint32_t)l[3] << 16));
+    for (int q = 0; q < 4; ++q) s[q] *= down;
     const float up = __uint_as_float((uint32_t)(127 + ex) << 23);
-    if constexpr (ALONE) {
-      *reinterpret_cast<uint2*>(hi + j) = hv;
-      *reinterpret_cast<uint2*>(lo + j) = lv;
-      if (j == 0) back[0] = up;
-    } else {
 #pragma unroll
-      for (int c = 0; c < AD_CTAS; ++c) {
-        st_cluster2(cluster_addr(hi + r * RP + j, c), hv);
-        st_cluster2(cluster_addr(lo + r * RP + j, c), lv);
-        if (j == 0) st_cluster1(cluster_addr(back + r, c), up);
+    for (int p = 0; p < PARTS; ++p) {
+      if (p >= parts) break;
+      uint16_t h[4];
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        h[q] = to16<F16>(s[q]);
+        const float rest = s[q] - from16<F16>(h[q]);
+        s[q] = fabsf(rest) < 1.f ? rest : 0.f;                             // an infinity or NaN stays in the first part alone
+      }
+      const uint2 hv = make_uint2(h[0] | ((uint32_t)h[1] << 16), h[2] | ((uint32_t)h[3] << 16));
+      uint16_t* dst = low + (p * ROWS + r) * RP + j;
+      if constexpr (ALONE) {
+        *reinterpret_cast<uint2*>(dst) = hv;
+      } else {
+#pragma unroll
+        for (int c = 0; c < AD_CTAS; ++c) st_cluster2(cluster_addr(dst, c), hv);
+      }
+    }
+    if (j == 0) {
+      if constexpr (ALONE) {
+        back[0] = up;
+      } else {
+#pragma unroll
+        for (int c = 0; c < AD_CTAS; ++c) st_cluster1(cluster_addr(back + r, c), up);
       }
     }
   }
@@ -436,12 +446,12 @@ adapters_kernel(AdArgs g) {
         for (int m = 0; m < MT; ++m) {
           if (16 * m >= cnt) break;
           const int ra = (ALONE ? 0 : 16 * m + gq) * RP + 16 * ks + 4 * t, rb = ALONE ? ra : ra + 8 * RP;
-          const uint2 ha = *reinterpret_cast<const uint2*>(hi + ra), hb = *reinterpret_cast<const uint2*>(hi + rb);
-          const uint2 la = *reinterpret_cast<const uint2*>(lo + ra), lb = *reinterpret_cast<const uint2*>(lo + rb);
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            mma16<F16>(d[m][j], la.x, lb.x, la.y, lb.y, bv[c][ks][j].x, bv[c][ks][j].y);
-            mma16<F16>(d[m][j], ha.x, hb.x, ha.y, hb.y, bv[c][ks][j].x, bv[c][ks][j].y);
+          for (int p = PARTS - 1; p >= 0; --p) {                           // the smallest first
+            if (p >= parts) continue;
+            const uint2 sa = *reinterpret_cast<const uint2*>(low + p * ROWS * RP + ra), sb = *reinterpret_cast<const uint2*>(low + p * ROWS * RP + rb);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) mma16<F16>(d[m][j], sa.x, sb.x, sa.y, sb.y, bv[c][ks][j].x, bv[c][ks][j].y);
           }
         }
       if (c == CH - 1 && c0 + CH * STRIDE < N) load_b(c0 + CH * STRIDE);

@@ -143,9 +143,7 @@ class Exl3Linear:
             y += self.bias.float()
         want = out_dtype or (out.dtype if out is not None else x.dtype)
         if adapters is not None:
-            if out is None and want in low_rank.ROW_TYPES:
-                return low_rank.add_checked(x, adapters, plan, y, None, want)
-            low_rank.add_checked(x, adapters, plan, y, y, None)
+            y = low_rank.add_checked(x, adapters, plan, y, None, want if want in low_rank.ROW_TYPES else None)
         if out is None:
             return y.to(want)
         out.copy_(y)

@@ -58,9 +58,9 @@ def plan_of(ids, count):
 def reference(x, ad, ids, base, out_type):
     """The formula in 64 bits, and how far the kernel's rows may be: the low-rank sums are off by at most K truncated fp32
     steps of 2^-23 of the sum of magnitudes, and one for the scale; they are split into two parts of t bits each with a
-    rest below half a step of the second, after scaling the row's largest value into [1, 2): 2^-16 (bf16: 8 + 8 bits) of a
-    value, or for fp16 2^-22 of it or, where the second part is below fp16's normal range, 2^-25 of the row's largest;
-    the columns' sums add 2 R steps, the base one; then one rounding of half a step."""
+    rest below half a step of the second, after scaling the row's largest value into [1, 2): 2^-16 (bf16: 8 + 8 bits; with a
+    third part under fp32 rows 2^-24) of a value, or for fp16 2^-22 of it or, where the second part is below fp16's normal
+    range, 2^-25 of the row's largest; the columns' sums add 3 R steps, the base one; then one rounding of half a step."""
 
     want, room = base.double().clone(), torch.zeros(base.shape, dtype=torch.float64, device=DEV)
     k, rank = ad.k, ad.a.shape[1]
@@ -70,11 +70,11 @@ def reference(x, ad, ids, base, out_type):
         a, b, sc = ad.a[i].double(), ad.b[i].double(), ad.scale[i].double()
         s, mag = sc * (a @ x[m].double()), sc.abs() * (a.abs() @ x[m].double().abs())
         es = mag * (k + 1) * 2.0 ** -23
-        es = es + (s.abs() * 2.0 ** -16 if ad.dtype == BF else s.abs() * 2.0 ** -22 + s.abs().max() * 2.0 ** -25)
+        es = es + (s.abs() * 2.0 ** (-24 if out_type == F32 else -16) if ad.dtype == BF else s.abs() * 2.0 ** -22 + s.abs().max() * 2.0 ** -25)
         delta = b @ s
         want[m] += delta
         parts = b.abs() @ (s.abs() + es)
-        room[m] = (b.abs() @ es + parts * 2 * rank * 2.0 ** -23 + want[m].abs() * 2.0 ** -24) * 1.01
+        room[m] = (b.abs() @ es + parts * 3 * rank * 2.0 ** -23 + want[m].abs() * 2.0 ** -24) * 1.01
     if out_type != F32:
         room = room + want.abs() * torch.finfo(out_type).eps / 2 + 2.0 ** -25
     return want, room
