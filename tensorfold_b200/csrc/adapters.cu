@@ -466,6 +466,8 @@ adapters_kernel(AdArgs g) {
           const int have = min(8, N - cl);
           float v[8];
           ad_widen(pb[c][m][h], g.base_type, wide_base && have == 8, v);
+          if (!ALONE && cl + STRIDE < N)                                   // the next block's, as soon as its place is free
+            ad_load8(g.base, g.base_type, row[r] * g.base_stride + cl + STRIDE, wide_base && cl + STRIDE + 8 <= N, N - cl - STRIDE, pb[c][m][h]);
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             v[2 * j] = fmaf(d[m][j][2 * h], bk, v[2 * j]);
@@ -474,7 +476,7 @@ adapters_kernel(AdArgs g) {
           ad_store8(g.out, g.out_type, wide_out, row[r] * g.out_stride + cl, have, v);
         }
     }
-    if (c0 + CH * STRIDE < N) load_base(c0 + CH * STRIDE);
+    if (ALONE && c0 + CH * STRIDE < N) load_base(c0 + CH * STRIDE);
   }
   if constexpr (ALONE) cluster_wait();                                     // nobody reads this CTA's sums any more
 }
