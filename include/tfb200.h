@@ -332,7 +332,7 @@ int tfb_unpack16(const void* packed, void* m0, void* m1, int experts, int n, int
 
 /* The grouped product over a plan (tfb_plan, tfb_select_plan, tfb_route) whose items hold at most `tile` pairs (1..256):
  * row p of out = f(x[p / slots] times the rows of expert e(p)), or x[p] when slots is 0; rows of pairs that are not in the
- * plan are left as they are.  epi: 0 fp32 out, 1 relu^2, 2 SwiGLU over (gate, up) clipped at limit when limit > 0, 3 the
+ * plan, and of pairs that the plan has but these rows have not, are left as they are.  epi: 0 fp32 out, 1 relu^2, 2 SwiGLU over (gate, up) clipped at limit when limit > 0, 3 the
  * sum; 1 to 3 rounded once to the weights' type (fp16 != 0: fp16, else bf16), which x has too.  x: x_rows rows of k inputs,
  * x_stride elements apart, 16-byte aligned; w: `experts` packed matrices.  max_items: an upper bound of the plan's items.  A pair's bits depend on its own
  * row alone. */

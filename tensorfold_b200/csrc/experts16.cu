@@ -364,6 +364,7 @@ g16_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ CUt
   const int units = __shfl_sync(0xffffffffu, ld_any(counts), 0) * nct;
   bool ok = true;
   auto item = [&](int u) { return min(u, units - 1) / nct; };              // of the next unit, or any where there is none
+  auto known = [&](int p) { return p < pairs ? p : -1; };                  // a plan of more rows than this call has
 
   if (units == 0) {
   } else if (warp == SH::A_WARP) {
@@ -393,6 +394,11 @@ g16_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ CUt
         __syncwarp();
         at.next(STAGES);
       }
+    }
+    // once around: the last MMAs' arrivals on `empty` land before the CTA's shared memory goes to another
+    for (int i = 0; i < STAGES && ok; ++i) {
+      ok = mbar_wait_warp(empty + at.s, at.ph ^ 1);
+      at.next(STAGES);
     }
     if (!ok) at.drain(full, STAGES, cta == 0);
     __syncwarp();
@@ -460,7 +466,7 @@ g16_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ CUt
           ok = mbar_wait_warp(full + at.s, at.ph);
           if (!ok) break;
           tc_fence_after();
-            if (elect_one()) {
+          if (elect_one()) {
             const uint32_t off = (uint32_t)(at.s * SH::STAGE) >> 4;
 #pragma unroll
             for (int ks = 0; ks < 4; ++ks) umma_ss<CG>(acc, a0 + off + 2 * ks, b0 + off + 2 * ks, idesc, (f | ks) ? 1u : 0u);
@@ -481,7 +487,7 @@ g16_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ CUt
     for (int u = u0; u < units && ok; u += du, ++n) {
       const int r0 = ((u - u / nct * nct) * CG + cta) * W16_ROWS, have = min(cnt, MAXP);
       int* pair = table + (n & 1) * MAXP;
-      for (int i = tid; i < ((have + 31) & ~31); i += SH::EPI_WARPS * 32) pair[i] = i < have ? ld_any(members + first + i) : -1;
+      for (int i = tid; i < ((have + 31) & ~31); i += SH::EPI_WARPS * 32) pair[i] = i < have ? known(ld_any(members + first + i)) : -1;
       first = ld_any(items + 3 * item(u + du) + 1);
       cnt = ld_any(items + 3 * item(u + du) + 2);
       asm volatile("bar.sync 1, %0;\n" ::"n"(SH::EPI_WARPS * 32) : "memory");
@@ -662,7 +668,8 @@ extern "C" int tfb_unpack16(const void* packed, void* m0, void* m1, int experts,
                     "unpack16");
 }
 
-// `picks` null: over the plan in items, counts and members; else these are not read and the launch sorts the `pairs` picks.
+// `picks` null: over the plan in items, counts and members, the call's `pairs` of it; else these are not read and the launch
+// sorts the `pairs` picks.
 static int experts16_run(int epi, int fp16, const void* x, int64_t x_stride, int64_t x_rows, int slots, const void* w, int experts,
                          int k, int n, const int32_t* items, const int32_t* counts, const int32_t* members, const int32_t* picks,
                          int pairs, void* out, float limit, int64_t max_items, int tile, cudaStream_t st) {
@@ -710,8 +717,10 @@ extern "C" int tfb_experts16(int epi, int fp16, const void* x, int64_t x_stride,
   TFB_REQUIRE(slots >= 0 && max_items >= 0, "experts16: bad slots or item count");
   TFB_REQUIRE(epi >= EPI_F32 && epi <= EPI_BF16, "experts16: no kernel for epilogue %d", epi);
   if (max_items == 0 || x_rows == 0) return TFB_OK;
-  return experts16_run(epi, fp16, x, x_stride, x_rows, slots, w, experts, k, n, items, counts, members, nullptr, 0, out, limit,
-                       max_items, tile, static_cast<cudaStream_t>(stream));
+  const int64_t pairs = slots ? x_rows * slots : x_rows;
+  TFB_REQUIRE(pairs < (int64_t(1) << 31), "experts16: 2^31 pairs or more");
+  return experts16_run(epi, fp16, x, x_stride, x_rows, slots, w, experts, k, n, items, counts, members, nullptr, (int)pairs, out,
+                       limit, max_items, tile, static_cast<cudaStream_t>(stream));
 }
 
 // The whole routed block behind one call: plan, gate/up, down and the weighted sum over the slots whose pick names an expert.

@@ -146,7 +146,8 @@ def _adapted(x: torch.Tensor, q: Q4, f32: bool, out: torch.Tensor | None, prefil
     want = torch.float32 if f32 else torch.bfloat16
     if out is not None and (out.shape != (x.shape[0], q.n) or out.dtype != want or not out.is_contiguous()):
         raise ValueError(f"out must be contiguous ({x.shape[0]}, {q.n}) {want}")
-    return low_rank.add_checked(x, adapters, plan, _run(x, q, True, None, prefill), out, want)
+    base = torch.empty_strided((x.shape[0], q.n), (q.n, 1), dtype=torch.float32, device=x.device) if q.n == q.n_pad else None
+    return low_rank.add_checked(x, adapters, plan, _run(x, q, True, base, prefill), out, want)
 
 
 def matmul(x: torch.Tensor, q: Q4, xs: torch.Tensor | None = None, *, sk: int | None = None, f32: bool = False,

@@ -289,6 +289,28 @@ def test_few_pairs_need_no_plan(rows, slots, count):
     assert torch.equal(got, want[:rows]) and torch.equal(want[-rows:], want[:rows])
 
 
+@pytest.mark.parametrize("tile", [32, 64, 256])
+def test_a_plan_of_more_rows_than_the_call(tile):
+    """Fewer rows than were routed: their pairs' rows, and nothing behind them."""
+
+    from tensorfold_b200 import experts, experts16
+
+    case = (BF, True, 0.0, 3, 136, 72, 2, 90)
+    up, down = weights(case, 77)
+    ex = experts16.make(up, down)
+    x, picks = normal(4, 90, 136), picks_of(90, 2, 3)
+    act, y = run(ex, x, picks)
+    plan = experts16.Plan(90, 2, 3, DEV)
+    plan.decode_tile = tile
+    experts.route(picks, plan)
+    got = torch.full((180, 72), 55.0, dtype=BF, device=DEV)
+    rows = torch.full((180, 136), 55.0, device=DEV)
+    experts16.gate_up(x[:41], ex, plan, got[:82], 41)
+    experts16.down(got[:82], ex, plan, rows[:82], 41)
+    assert torch.equal(got[:82], act[:82]) and (got[82:] == 55).all()
+    assert torch.equal(rows[:82], y[:82]) and (rows[82:] == 55).all()
+
+
 def test_a_plan_without_pairs_and_calls_without_rows():
     from tensorfold_b200 import experts16, moe
 
