@@ -202,7 +202,8 @@ struct AdShape {
   static constexpr int KU = NT > 1 ? (RT <= 2 ? 2 : 1) : (RT <= 2 ? 4 : RT == 4 ? 2 : 1);   // steps of 32 inputs loaded at once
   static constexpr int CH = ALONE && RT <= 2 ? 2 : 1;   // blocks of columns loaded at once
   static constexpr int PART = AD_WARPS * ROWS * PITCH * 4;                 // float part[warp][row][PITCH]; the sum in warp 0's
-  static constexpr int LOW = ROWS * RP * 2;                                // a part of the low-rank rows, [row][RP]
+  static constexpr int LP = RT == 1 ? RP : RP + 16;                        // a tile's rows then spread over the banks
+  static constexpr int LOW = ROWS * LP * 2;                                // a part of the low-rank rows, [row][LP]
   static constexpr int LOW_OFFSET = PART;
   static constexpr int BACK_OFFSET = LOW_OFFSET + 3 * LOW;                 // float back[row]: the row's scaling undone
   static constexpr int ROW_OFFSET = BACK_OFFSET + ROWS * 4;                // int row[ROWS]
@@ -215,7 +216,7 @@ template <int RT, int NT, bool F16>
 __global__ void __launch_bounds__(AD_WARPS * 32, RT == 1 ? 5 : RT == 2 ? 4 : RT == 4 ? 3 : 1)
 adapters_kernel(AdArgs g) {
   using SH = AdShape<RT, NT>;
-  constexpr int ROWS = SH::ROWS, RP = SH::RP, PITCH = SH::PITCH, MT = SH::MT, QUADS = SH::QUADS, KU = SH::KU, CH = SH::CH;
+  constexpr int ROWS = SH::ROWS, RP = SH::RP, PITCH = SH::PITCH, LP = SH::LP, MT = SH::MT, QUADS = SH::QUADS, KU = SH::KU, CH = SH::CH;
   constexpr bool ALONE = SH::ALONE;
   constexpr int THREADS = AD_WARPS * 32, STRIDE = AD_CTAS * AD_WARPS * 32;   // columns the cluster forms at a time
   extern __shared__ __align__(16) uint8_t ad_smem[];
@@ -408,7 +409,7 @@ adapters_kernel(AdArgs g) {
         s[q] = fabsf(rest) < 1.f ? rest : 0.f;                             // an infinity or NaN stays in the first part alone
       }
       const uint2 hv = make_uint2(h[0] | ((uint32_t)h[1] << 16), h[2] | ((uint32_t)h[3] << 16));
-      uint16_t* dst = low + (p * ROWS + r) * RP + j;
+      uint16_t* dst = low + (p * ROWS + r) * LP + j;
       if constexpr (ALONE) {
         *reinterpret_cast<uint2*>(dst) = hv;
       } else {
@@ -445,11 +446,11 @@ adapters_kernel(AdArgs g) {
 #pragma unroll
         for (int m = 0; m < MT; ++m) {
           if (16 * m >= cnt) break;
-          const int ra = (ALONE ? 0 : 16 * m + gq) * RP + 16 * ks + 4 * t, rb = ALONE ? ra : ra + 8 * RP;
+          const int ra = (ALONE ? 0 : 16 * m + gq) * LP + 16 * ks + 4 * t, rb = ALONE ? ra : ra + 8 * LP;
 #pragma unroll
           for (int p = PARTS - 1; p >= 0; --p) {                           // the smallest first
             if (p >= parts) continue;
-            const uint2 sa = *reinterpret_cast<const uint2*>(low + p * ROWS * RP + ra), sb = *reinterpret_cast<const uint2*>(low + p * ROWS * RP + rb);
+            const uint2 sa = *reinterpret_cast<const uint2*>(low + p * ROWS * LP + ra), sb = *reinterpret_cast<const uint2*>(low + p * ROWS * LP + rb);
 #pragma unroll
             for (int j = 0; j < 4; ++j) mma16<F16>(d[m][j], sa.x, sb.x, sa.y, sb.y, bv[c][ks][j].x, bv[c][ks][j].y);
           }
