@@ -108,7 +108,7 @@ struct G16Shape {
   static constexpr int TOTAL = TMEM_OFFSET + 16 + 1024;                    // + slack to align the tiles to 1024 bytes
   static constexpr int ACC_COLS = MAXP;                                    // tensor memory: two accumulators
   static constexpr int STEP = 16 * CG;                                     // N is a multiple of it
-  static constexpr int LANES = (MAXP / CG / 4 + B_WARPS - 1) / B_WARPS;                // lanes of a gathering warp with a group of rows
+  static constexpr int LANES = (MAXP / CG / 4 + B_WARPS - 1) / B_WARPS;    // lanes of a gathering warp with a group of rows
   static_assert(TOTAL <= 227 * 1024, "one CTA's shared memory");
   static_assert(ACC_COLS >= 32 && 2 * ACC_COLS <= 512 && LANES >= 1 && LANES <= 32, "tensor memory; the gathers");
 };
@@ -310,9 +310,9 @@ struct RingAt {                                     // a walk around the ring of
 // rows took 2 us in which the ring ran dry.
 template <int CG, int M, int EPI, bool F16, int MAXP>
 __global__ void __launch_bounds__(G16Shape<CG, MAXP>::THREADS, 1)
-g16_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ CUtensorMap wmap, int slots, const uint8_t* __restrict__ W, int K, int N,
-           const int* items, const int* counts, const int* members, const int* picks, int pairs, int experts, int tile,
-           void* __restrict__ out, float limit) {
+g16_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ CUtensorMap wmap, int slots,
+           const uint8_t* __restrict__ W, int K, int N, const int* items, const int* counts, const int* members, const int* picks,
+           int pairs, int experts, int tile, void* __restrict__ out, float limit) {
   using SH = G16Shape<CG, MAXP>;
   constexpr int STAGES = SH::STAGES, B_WARPS = SH::B_WARPS;
   extern __shared__ uint8_t smem_raw[];
