@@ -89,13 +89,14 @@ def test_item_sizes():
 def test_cpu_tensors_are_refused():
     from tensorfold_b200 import adapters, experts16, moe
 
-    ex = SimpleNamespace(up=torch.zeros((2, 16, 64), dtype=BF), down=torch.zeros((2, 16, 64), dtype=BF), width=16, dims=16,
-                         swiglu=False, limit=0.0, count=2, dtype=BF)
+    ex = experts16.Experts16(torch.zeros((2, 16, 64), dtype=BF), torch.zeros((2, 16, 64), dtype=BF), 16, 16, False)
     plan = experts16.Plan(4, 1, 2, "cpu")
     with pytest.raises(ValueError, match="CUDA"):
         experts16.gate_up(torch.zeros((4, 16), dtype=BF), ex, plan, torch.zeros((4, 16), dtype=BF), 4)
     with pytest.raises(ValueError, match="CUDA"):
         moe.picked(torch.zeros((4, 16), dtype=BF), ex, torch.zeros((4, 1), dtype=torch.int32), torch.zeros((4, 1)))
+    with pytest.raises(ValueError, match="4-bit experts"):
+        moe.picked(torch.zeros((4, 16), dtype=BF), SimpleNamespace(), torch.zeros((4, 1), dtype=torch.int32), torch.zeros((4, 1)))
     with pytest.raises(ValueError, match="CUDA"):
         adapters.route(torch.zeros((4,), dtype=torch.int32), adapters.Plan(4, 2, "cpu"))
     ad = adapters.Adapters(2, 8, 16, 16, device="cpu")

@@ -352,6 +352,28 @@ def test_the_layer_takes_either_kind_of_experts(pdl):
         assert (prompt.double() - want).norm() <= 2.0 ** -7 * want.norm()   # and one of the rows
 
 
+@pytest.mark.parametrize("prefill", [False, True])
+@pytest.mark.parametrize("shared", [False, True])
+def test_picked_on_4_bit_experts(prefill, shared):
+    """A 4-bit layer's own picks and weights through ``picked``: the layer's bits; slots that take no part."""
+
+    from tensorfold_b200 import experts, moe, synthetic
+
+    shape = synthetic.SMALL_SHARED if shared else synthetic.SMALL
+    gate, up, down = synthetic.affine_layer(shape, DEV)
+    layer = moe.Routed(synthetic.router_rows(shape, DEV), experts.make([gate, up], down, 64), shape.top_k, shared=shared)
+    x = synthetic.activations(shape, 21, DEV)
+    buf = moe.MoEBuffers(21, moe._Shape(layer), DEV, prefill=prefill, shared=shared)
+    want = torch.empty((21, shape.dims), dtype=BF, device=DEV)
+    moe.layer(x, layer, buf, want)
+    pick, wts = buf.pick[:21].contiguous(), buf.wts[:21].contiguous()
+    mine = moe.buffers(layer.experts, 21, pick.shape[1], prefill=prefill)
+    assert torch.equal(moe.picked(x, layer.experts, pick, wts, buf=mine), want)
+    pick[3], wts[3] = -1, float("nan")
+    got = moe.picked(x, layer.experts, pick, wts, buf=mine)
+    assert (got[3] == 0).all() and torch.equal(got[:3], want[:3]) and torch.equal(got[4:], want[4:])
+
+
 def test_graph_replays_follow_the_picks_on_their_own_scratch():
     """Two captured layers with buffers of their own, replayed in turn on other picks and rows, on another stream."""
 
