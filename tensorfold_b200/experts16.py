@@ -102,9 +102,32 @@ def make(up: list[torch.Tensor], down: torch.Tensor, *, limit: float = 0.0) -> E
     return Experts16(pack(*up), pack(down), width, dims, len(up) == 2, float(limit))
 
 
+def _check_packed(w: torch.Tensor, name: str, experts: int, rows: int, k: int, like: torch.Tensor) -> None:
+    """The kernel reads a packed tensor by its address alone: expert e's rows at e * rows * k."""
+
+    want = (experts, rows, -(-k // 64) * 64)
+    if tuple(w.shape) != want or w.dtype not in DTYPES or not w.is_contiguous() or w.data_ptr() % 16:
+        raise ValueError(f"{name}: packed weights {list(want)} in bf16 or fp16, contiguous and 16-byte aligned, not {w.dtype} "
+                         f"{tuple(w.shape)} with strides {w.stride()}")
+    if w.dtype != like.dtype or w.device != like.device:
+        raise ValueError(f"{name}: every projection must share one dtype and device")
+
+
+def check_up(ex: Experts16) -> None:
+    _check_packed(ex.up, "up", ex.count, _rows(2 if ex.swiglu else 1, ex.width), ex.dims, ex.up)
+
+
+def check_down(ex: Experts16) -> None:
+    """``down`` holds as many experts as ``up``, in its type and on its device."""
+
+    _check_packed(ex.down, "down", ex.count, _rows(1, ex.dims), ex.width, ex.up)
+
+
 def unpack(ex: Experts16) -> tuple[list[torch.Tensor], torch.Tensor]:
     """``make``'s inverse, bit for bit: ([gate, up] or [up], down)."""
 
+    check_up(ex)
+    check_down(ex)
     return (_unpack(ex.up, 2 if ex.swiglu else 1, ex.width, ex.dims), _unpack(ex.down, 1, ex.dims, ex.width)[0])
 
 
@@ -141,8 +164,6 @@ def _run(epi: int, x: torch.Tensor, slots: int, w: torch.Tensor, k: int, n: int,
         raise ValueError(f"out: contiguous {want} rows of {n} columns, one a pair")
     if out.device != device or w.device != device or plan.members.device != device:
         raise ValueError("x, the experts, the plan and out must be on one device")
-    if not w.is_contiguous():
-        raise ValueError("w must be contiguous")
     if plan.hot or plan.prefill or not grouped.TILE <= plan.tile <= ITEM:
         raise ValueError(f"a plan with items of {grouped.TILE} to {ITEM} pairs (experts16.Plan)")
     if rows < 0 or rows > plan.rows:
@@ -162,6 +183,7 @@ def gate_up(x: torch.Tensor, ex: Experts16, plan: grouped.Plan, out: torch.Tenso
     """x [R, D] (the experts' type, unit-stride rows) -> out [R * slots, NI], each pair's activation in the same type."""
 
     _fits(ex, plan)
+    check_up(ex)
     _run(2 if ex.swiglu else 1, x, plan.slots, ex.up, ex.dims, ex.width, plan, out, ex.limit, rows)
 
 
@@ -169,4 +191,5 @@ def down(act: torch.Tensor, ex: Experts16, plan: grouped.Plan, out: torch.Tensor
     """act [R * slots, NI] -> out [R * slots, D] per pair: fp32, or the experts' type when ``out`` has it."""
 
     _fits(ex, plan)
+    check_down(ex)
     _run(0 if out.dtype == torch.float32 else 3, act, 0, ex.down, ex.width, ex.dims, plan, out, 0.0, rows)

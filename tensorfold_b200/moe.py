@@ -321,6 +321,9 @@ def picked(x: torch.Tensor, ex, picks: torch.Tensor, wts: torch.Tensor, *, buf: 
 
     if not isinstance(ex, (grouped.Experts, experts16.Experts16)):
         raise ValueError("picked: affine 4-bit experts (experts.Experts) or 16-bit ones (experts16.Experts16)")
+    if isinstance(ex, experts16.Experts16):
+        experts16.check_up(ex)
+        experts16.check_down(ex)
     if x.dim() != 2 or picks.dim() != 2 or x.shape[0] != picks.shape[0] or x.shape[1] != ex.dims or picks.shape[1] < 1:
         raise ValueError(f"picked: x [R, {ex.dims}] and picks [R, slots], not {tuple(x.shape)} and {tuple(picks.shape)}")
     rows, slots = picks.shape
