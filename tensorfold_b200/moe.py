@@ -312,6 +312,16 @@ def buffers(ex, rows: int, slots: int, *, prefill: bool = False) -> MoEBuffers:
     return MoEBuffers(rows, _Picked(ex, slots), ex.up.device, prefill=prefill, shared=False, dtype=_weights_type(ex))
 
 
+def _check_blocks(ex: grouped.Experts) -> None:
+    """4-bit experts' blocks are read by their address too: ``down`` holds as many experts as ``up``, each of the layer's size."""
+
+    n, k = ex.width // grouped.COLS, ex.dims // ex.gs
+    for w, name, outer in ((ex.up, "up", (ex.count, n, k)), (ex.down, "down", (ex.count, ex.dims // grouped.COLS, ex.width // ex.gs))):
+        if tuple(w.shape[:3]) != outer or w.shape[-1] != grouped.BLOCK or w.dtype != torch.int32 or not w.is_contiguous() \
+                or w.device != ex.up.device:
+            raise ValueError(f"{name}: contiguous int32 blocks {list(outer)} on the experts' device, not {w.dtype} {tuple(w.shape)}")
+
+
 def picked(x: torch.Tensor, ex, picks: torch.Tensor, wts: torch.Tensor, *, buf: MoEBuffers | None = None,
            out: torch.Tensor | None = None) -> torch.Tensor:
     """The experts and weights a caller's own routing picked: x [R, D], picks [R, slots] int32, wts [R, slots] fp32 ->
@@ -324,6 +334,8 @@ def picked(x: torch.Tensor, ex, picks: torch.Tensor, wts: torch.Tensor, *, buf: 
     if isinstance(ex, experts16.Experts16):
         experts16.check_up(ex)
         experts16.check_down(ex)
+    else:
+        _check_blocks(ex)
     if x.dim() != 2 or picks.dim() != 2 or x.shape[0] != picks.shape[0] or x.shape[1] != ex.dims or picks.shape[1] < 1:
         raise ValueError(f"picked: x [R, {ex.dims}] and picks [R, slots], not {tuple(x.shape)} and {tuple(picks.shape)}")
     rows, slots = picks.shape

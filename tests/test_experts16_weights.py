@@ -85,3 +85,23 @@ def test_a_strided_shard_is_refused_and_its_copy_runs():
     copy = experts16.Experts16(shard.up.contiguous(), shard.down.contiguous(), 24, 72, True)
     mine = experts16.make([m[::2].contiguous() for m in up], down[::2].contiguous())
     assert torch.equal(moe.picked(x, copy, picks, wts), moe.picked(x, mine, picks, wts))
+
+
+BAD_BLOCKS = {"down-shorter": lambda ex: setattr(ex, "down", ex.down[:3]), "down-narrow": lambda ex: setattr(ex, "down", ex.down[:, :-1].contiguous()),
+              "down-strided": lambda ex: setattr(ex, "down", torch.cat([ex.down, ex.down])[::2]),
+              "down-elsewhere": lambda ex: setattr(ex, "down", ex.down.to("meta")), "up-strided": lambda ex: setattr(ex, "up", torch.cat([ex.up, ex.up])[::2]),
+              "up-groups": lambda ex: setattr(ex, "dims", 192), "down-type": lambda ex: setattr(ex, "down", ex.down.float())}
+
+
+@pytest.mark.parametrize("kind", BAD_BLOCKS)
+def test_picked_refuses_4_bit_blocks_that_do_not_fit_together(kind):
+    from tensorfold_b200 import experts, moe
+
+    ex = experts.Experts(torch.zeros((4, 2, 2, 2, experts.BLOCK), dtype=torch.int32),
+                         torch.zeros((4, 4, 1, 1, experts.BLOCK), dtype=torch.int32), 64, 64, 128)
+    picks, wts = torch.zeros((4, 1), dtype=torch.int32), torch.zeros((4, 1))
+    with pytest.raises(ValueError, match="CUDA"):
+        moe.picked(torch.zeros((4, 128), dtype=BF), ex, picks, wts)
+    BAD_BLOCKS[kind](ex)
+    with pytest.raises(ValueError, match="contiguous int32 blocks"):
+        moe.picked(torch.zeros((4, ex.dims), dtype=BF), ex, picks, wts)
