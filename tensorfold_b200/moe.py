@@ -8,6 +8,7 @@ slot for layers without a shared expert.
 
 from __future__ import annotations
 
+import threading
 from dataclasses import dataclass
 
 import torch
@@ -282,19 +283,45 @@ def _weights_type(ex) -> torch.dtype | None:
     return ex.dtype if isinstance(ex, experts16.Experts16) else None
 
 
-_scratch: dict[tuple, MoEBuffers] = {}
+SCRATCH_KEPT = 8         # sets of scratch ``run`` keeps for one shape of layer: the streams and threads that last asked first
+
+_scratch: dict[tuple, dict[tuple, MoEBuffers]] = {}
+
+
+def _capturing(device: torch.device) -> bool:
+    with _lib.on(device):
+        return torch.cuda.is_current_stream_capturing()
+
+
+def _scratch_of(rows: int, m: Routed, prefill: bool, device: torch.device) -> MoEBuffers:
+    """``run``'s scratch.  A call's launches hand their results on through it, so two calls may share it only if one's launches
+    are enqueued behind the other's: it belongs to a stream and, since two threads may enqueue in turn on one stream, to a
+    thread.  A captured call's belongs to its graph, which may be replayed beside anything."""
+
+    dtype = _weights_type(m.experts)
+
+    def make() -> MoEBuffers:
+        return MoEBuffers(size, _Shape(m), device, prefill=prefill, shared=m.shared, dtype=dtype)
+
+    size = 1 << max(4, (rows - 1).bit_length())                 # scratch per power of two, reused by every layer
+    if _capturing(device):
+        return make()
+    key = (size, m.count, m.top_k, m.experts.width, m.experts.dims, prefill, m.shared, device, dtype)
+    kept = _scratch.setdefault(key, {})
+    who = (_lib.stream(device), threading.get_ident())
+    buf = kept.get(who)
+    if buf is None:
+        while len(kept) >= SCRATCH_KEPT:                        # its memory goes back to its stream, behind what runs there
+            kept.pop(list(kept)[0], None)
+        buf = kept[who] = make()
+    return buf
 
 
 def run(x: torch.Tensor, m: Routed, *, prefill: bool = False) -> torch.Tensor:
     """x [R, D] bf16 -> [R, D] bf16: its top-k experts by renormalized softmax weight (plus the shared expert)."""
 
     rows = x.shape[0]
-    size = 1 << max(4, (rows - 1).bit_length())                 # scratch per power of two, reused by every layer
-    dtype = _weights_type(m.experts)
-    key = (size, m.count, m.top_k, m.experts.width, m.experts.dims, prefill, m.shared, x.device, dtype)
-    buf = _scratch.get(key)
-    if buf is None:
-        buf = _scratch[key] = MoEBuffers(size, _Shape(m), x.device, prefill=prefill, shared=m.shared, dtype=dtype)
+    buf = _scratch_of(rows, m, prefill, x.device)
     out = torch.empty((rows, m.experts.dims), dtype=torch.bfloat16, device=x.device)
     layer(x.contiguous(), m, buf, out)
     return out
