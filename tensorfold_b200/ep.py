@@ -28,6 +28,16 @@ import torch.distributed as dist
 from . import _lib
 
 
+def _check_kind(*experts) -> None:
+    """Before any window or buffer is made: the steps here run affine 4-bit experts (``PeerExl3ExpertParallel``: EXL3)."""
+
+    from . import experts as grouped
+
+    for ex in experts:
+        if ex is not None:
+            grouped.check_kind(ex)
+
+
 class CudaBackend:
     """This rank's share of a layer on its GPU: full router rows, its slice of the routed experts, the shared expert."""
 
@@ -36,6 +46,7 @@ class CudaBackend:
         from . import experts as grouped
         from . import moe
 
+        _check_kind(local_experts, shared_experts)
         self.moe, self.grouped = moe, grouped
         self.router_rows, self.local, self.top_k, self.experts = router_rows, local_experts, top_k, experts
         self.shared = shared_experts                      # an Experts object holding the one shared expert, or None
@@ -167,6 +178,7 @@ class GatheredExpertParallel:
         from . import experts as grouped
         from . import moe
 
+        _check_kind(local_experts)
         if reduce not in ("rows", "tokens"):
             raise ValueError("reduce must be 'rows' or 'tokens'")
         self.reduce = reduce
@@ -392,6 +404,7 @@ class PeerExpertParallel:
         from . import experts as grouped
         from . import moe
 
+        _check_kind(local_experts, shared_experts)
         self.moe, self.grouped = moe, grouped
         shared = shared_experts is not None
         self.win = w = PeerWindow(router_rows, experts, top_k, rows_local, local_experts.dims, shared, group,

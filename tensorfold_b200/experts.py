@@ -261,7 +261,7 @@ def _rejoin(plan, device) -> None:
         torch.cuda.current_stream(device).wait_event(plan.joined)
 
 
-def _check_kind(ex) -> None:
+def check_kind(ex) -> None:
     if not isinstance(ex, Experts):
         raise ValueError("affine 4-bit experts; those on 16-bit weights run through experts16")
 
@@ -296,7 +296,7 @@ def _run(epi: int, x: torch.Tensor, slots: int, w: torch.Tensor, kg: int, nb: in
 def gate_up(x: torch.Tensor, ex: Experts, plan: Plan, out: torch.Tensor, rows: int) -> None:
     """x [R, D] bf16 (unit-stride rows) -> out [R * slots, NI] bf16, each pair's activation."""
 
-    _check_kind(ex)
+    check_kind(ex)
     items = max_items(rows * plan.slots, plan.experts, plan.tile)
     epi = 2 if ex.swiglu else 1
     with _beside(plan, x.device) as hot:                     # the hot experts' pairs: other rows of the same output
@@ -312,7 +312,7 @@ def gate_up(x: torch.Tensor, ex: Experts, plan: Plan, out: torch.Tensor, rows: i
 def down(act: torch.Tensor, ex: Experts, plan: Plan, out: torch.Tensor, rows: int) -> None:
     """act [R * slots, NI] bf16 -> out [R * slots, D] per pair: fp32, or bf16 on a prefill plan when ``out`` is bf16."""
 
-    _check_kind(ex)
+    check_kind(ex)
     items = max_items(rows * plan.slots, plan.experts, plan.tile)
     epi = 3 if plan.prefill and out.dtype == torch.bfloat16 else 0
     with _beside(plan, act.device) as hot:
@@ -331,7 +331,7 @@ def down_combine(act: torch.Tensor, ex: Experts, plan: Plan, y: torch.Tensor, ro
     block stores a row's last slot.  Every (row, slot) pair must be in the plan; ``arrive`` is int32 scratch
     [R, D / 32], zero before the first call (a call leaves it zero)."""
 
-    _check_kind(ex)
+    check_kind(ex)
     if plan.prefill or plan.hot:
         raise ValueError("the fused combine follows the decode form of a plain plan")
     if y.dtype != torch.float32 or not y.is_contiguous() or y.shape[-1] != ex.dims:
