@@ -262,7 +262,9 @@ def _rejoin(plan, device) -> None:
 
 
 def check_kind(ex) -> None:
-    if not isinstance(ex, Experts):
+    """``Experts``, or any object with its fields."""
+
+    if not hasattr(ex, "gs"):
         raise ValueError("affine 4-bit experts; those on 16-bit weights run through experts16")
 
 
