@@ -4,7 +4,7 @@ A small reader of the safetensors container (8-byte little-endian header length,
 hands tensors to ``experts.make`` / ``exl3.experts.prepare`` / ``qmm.pack`` without a dequantised copy ever existing:
 * MLX affine 4-bit checkpoints - a layer's router rows and experts as ``moe.Routed`` (names as in
   ``src/tensorfold/families/qwen3_5_moe/cuda/weights.py:32-46``);
-* unquantised bf16 or fp16 checkpoints - a layer's router rows and experts as ``moe.Routed`` on ``experts16``;
+* unquantised bf16 checkpoints - a layer's router rows and experts as ``moe.Routed`` on ``experts16``;
 * EXL3 checkpoints - a group's ``trellis`` / ``suh`` | ``su`` / ``svh`` | ``sv`` / ``mcg`` | ``mul1`` parts
   (``src/tensorfold/cuda/exl3/format.py:226-267``) as ``Exl3Linear`` or as a layer's ``Exl3RoutedExperts``
   (``src/tensorfold/families/qwen4_exp/cuda/exl3.py:22-83``).
@@ -139,11 +139,17 @@ def affine_routed(ck: Checkpoint, prefix: str, top_k: int, device="cuda", gs: in
 def routed16(ck: Checkpoint, prefix: str, top_k: int, device="cuda"):
     """Layer ``prefix`` (ending in "mlp.") of an unquantised bf16 checkpoint as ``moe.Routed``: the names of
     ``affine_routed`` without scales and biases, the experts stacked ("switch_mlp.{proj}.weight") or one by one
-    ("experts.{e}.{proj}.weight"); the shared expert and its gate row last, where the layer has them."""
+    ("experts.{e}.{proj}.weight"); the shared expert and its gate row last, where the layer has them.  Experts of another
+    type are refused by the files' headers."""
 
     from . import experts16, moe
 
     shared = ck.has(prefix + "shared_expert_gate.weight")
+    for proj in PROJS:
+        each = [f"{prefix}experts.{e}.{proj}.weight" for e in range(ck.entry(prefix + "gate.weight")[4][0])]
+        for name in (f"{prefix}switch_mlp.{proj}.weight", f"{prefix}shared_expert.{proj}.weight", *each):
+            if ck.has(name) and ck.entry(name)[3] != "BF16":
+                raise ValueError(f"{name}: a routed layer runs in bf16, not {ck.entry(name)[3]}")
     rows = [ck.get(prefix + name + ".weight", device) for name in (("gate", "shared_expert_gate") if shared else ("gate",))]
     router = torch.cat(rows).to(torch.bfloat16).contiguous()
     count = rows[0].shape[0]
@@ -159,8 +165,6 @@ def routed16(ck: Checkpoint, prefix: str, top_k: int, device="cuda"):
         return torch.stack(mats)
 
     ex = experts16.make([table("gate_proj"), table("up_proj")], table("down_proj"))
-    if ex.dtype != torch.bfloat16:
-        raise ValueError(f"{prefix}: a routed layer runs in bf16, not {ex.dtype}")
     return moe.Routed(router, ex, int(top_k), shared=shared)
 
 
