@@ -140,7 +140,15 @@ def _end(t: torch.Tensor, m: int) -> int:
 
 
 def _overlap(a: torch.Tensor, b: torch.Tensor, m: int) -> bool:
-    return a.data_ptr() < _end(b, m) and b.data_ptr() < _end(a, m)
+    """Whether the first ``m`` rows of one may touch the other's; columns of their own of one buffer's rows do not."""
+
+    if a.data_ptr() >= _end(b, m) or b.data_ptr() >= _end(a, m):
+        return False
+    step = a.stride(0) * a.element_size()
+    if m == 1 or step != b.stride(0) * b.element_size() or step <= 0:
+        return True
+    at = (b.data_ptr() - a.data_ptr()) % step                                # b's columns within a's rows
+    return at < a.shape[1] * a.element_size() or at + b.shape[1] * b.element_size() > step
 
 
 def _rows_of(t: torch.Tensor, name: str, m: int, n: int, device: torch.device) -> tuple[int, int]:
@@ -201,7 +209,7 @@ def add_checked(x: torch.Tensor, ad: Adapters, plan: Plan, base: torch.Tensor, o
         out_type, out_step = _rows_of(out, "out", m, n, device)
         same = out.data_ptr() == base.data_ptr() and out_type == base_type and out_step == base_step
         if m and (_overlap(out, x, m) or not same and _overlap(out, base, m)):
-            raise ValueError("out may be base itself, but must not overlap x or a part of base")
+            raise ValueError("out may be base itself, but must not overlap x or a part of base (columns apart in one buffer's rows do not)")
     if m == 0:
         return out
     x_step = x.stride(0) if m > 1 else k
