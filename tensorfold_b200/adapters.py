@@ -69,11 +69,12 @@ class Adapters:
         if a.dim() != 2 or b.dim() != 2 or not 1 <= r <= self.rank or a.shape[1] != self.k or tuple(b.shape) != (self.n, r):
             raise ValueError(f"a [r, {self.k}] and b [{self.n}, r] with r <= {self.rank}, not {tuple(a.shape)} and "
                              f"{tuple(b.shape)}")
+        scale = float(scale)                                             # what is refused leaves the slot as it was
         self.a[i, :r].copy_(a)
         self.a[i, r:].zero_()
         self.b[i, :, :r].copy_(b)
         self.b[i, :, r:].zero_()
-        self.scale[i:i + 1].fill_(float(scale))
+        self.scale[i:i + 1].fill_(scale)
 
     def clear(self, i: int) -> None:
         """Empty slot ``i``: its rows then come out as the base alone."""
