@@ -39,6 +39,10 @@ int tfb_set_pdl(int on);
  * missing rank of NCCL.ready (src/tensorfold/cuda/comm.py:78-101). */
 int tfb_kernel_status(int* status, void* stream);
 
+/* The capture that `stream` records into, a number of its own for each capture of the process; 0 when it records none, all
+ * ones when CUDA cannot say.  For scratch that belongs to a graph. */
+uint64_t tfb_capture_id(void* stream);
+
 /* Milliseconds an expert-parallel barrier waits for the other ranks before it gives up (1 .. 600000; 1000 unless
  * set); returns the previous limit, or -1 with a message.  Read at launch (and at graph capture).  Counterpart of the
  * `timeout` of NCCL.ready (src/tensorfold/cuda/comm.py:78). */

@@ -4,7 +4,7 @@ from __future__ import annotations
 
 import contextlib
 import ctypes
-from ctypes import c_char_p, c_float, c_int, c_int64, c_void_p
+from ctypes import c_char_p, c_float, c_int, c_int64, c_uint64, c_void_p
 from functools import lru_cache
 from pathlib import Path
 
@@ -19,7 +19,8 @@ _RAW_STREAM = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 
 P, I, L, F = c_void_p, c_int, c_int64, c_float
 
-# name -> argument types (every entry point returns int status, except tfb_last_error / tfb_version / tfb_set_pdl)
+# name -> argument types (every entry point returns int status, except tfb_last_error / tfb_version / tfb_set_pdl and
+# tfb_capture_id)
 SIGNATURES: dict[str, tuple] = {
     "tfb_router": (P, L, P, P, I, I, I, P),
     "tfb_router_prompt": (P, L, P, P, I, I, I, P),
@@ -63,6 +64,7 @@ SIGNATURES: dict[str, tuple] = {
     "tfb_peer_push": (P, P, L, I, I, I, I, P, P),
     "tfb_window_picks": (P, P, I, I, P, P, I, P),
     "tfb_kernel_status": (P, P),
+    "tfb_capture_id": (P,),
 }
 
 
@@ -92,6 +94,7 @@ def lib() -> ctypes.CDLL:
         fn = getattr(handle, name)
         fn.argtypes = args
         fn.restype = c_int
+    handle.tfb_capture_id.restype = c_uint64
     # A layer of few tokens is a chain of short kernels, and the gaps between plain launches are a good part of it: with
     # programmatic launches steps in a row of one token through 128 experts take 24 us each instead of 27, of thirteen
     # tokens 62 instead of 74.  (A single step that is waited for gains about 1 %.)
@@ -128,6 +131,16 @@ def stream(device) -> int:
     if _RAW_STREAM is not None and device.index is not None:
         return _RAW_STREAM(device.index)                            # without a Stream object around it
     return torch.cuda.current_stream(device).cuda_stream
+
+
+def capture(stream: int) -> int:
+    """The capture into a CUDA graph that ``stream`` records, by a number of its own; 0 when it records none (the default
+    stream, handle 0, cannot)."""
+
+    got = lib().tfb_capture_id(stream) if stream else 0
+    if got == 2 ** 64 - 1:
+        raise RuntimeError(lib().tfb_last_error().decode("utf-8", "replace"))
+    return got
 
 
 def kernel_status(stream: int = 0) -> int:

@@ -64,3 +64,11 @@ extern "C" int tfb_kernel_status(int* status, void* stream) {
   *status = v;
   return TFB_OK;
 }
+
+// The capture that `stream` records into, an id of its own for each; 0 when it records none, -1 when CUDA cannot say.
+extern "C" uint64_t tfb_capture_id(void* stream) {
+  cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+  unsigned long long id = 0;
+  if (check_cuda(cudaStreamGetCaptureInfo(static_cast<cudaStream_t>(stream), &status, &id), "capture_id") != TFB_OK) return ~0ull;
+  return status == cudaStreamCaptureStatusNone ? 0 : id;
+}

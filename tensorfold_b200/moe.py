@@ -288,32 +288,24 @@ SCRATCH_KEPT = 8         # sets of scratch ``run`` keeps for one shape of layer:
 _scratch: dict[tuple, dict[tuple, MoEBuffers]] = {}
 
 
-def _capturing(device: torch.device) -> bool:
-    with _lib.on(device):
-        return torch.cuda.is_current_stream_capturing()
-
-
 def _scratch_of(rows: int, m: Routed, prefill: bool, device: torch.device) -> MoEBuffers:
     """``run``'s scratch.  A call's launches hand their results on through it, so two calls may share it only if one's launches
     are enqueued behind the other's: it belongs to a stream and, since two threads may enqueue in turn on one stream, to a
-    thread.  A captured call's belongs to its graph, which may be replayed beside anything."""
+    thread.  The calls of a capture share a set of their own, which the graph may use beside anything when it is replayed; it is
+    let go when the thread's next capture asks (the graph's own pool holds its memory)."""
 
     dtype = _weights_type(m.experts)
-
-    def make() -> MoEBuffers:
-        return MoEBuffers(size, _Shape(m), device, prefill=prefill, shared=m.shared, dtype=dtype)
-
     size = 1 << max(4, (rows - 1).bit_length())                 # scratch per power of two, reused by every layer
-    if _capturing(device):
-        return make()
     key = (size, m.count, m.top_k, m.experts.width, m.experts.dims, prefill, m.shared, device, dtype)
     kept = _scratch.setdefault(key, {})
-    who = (_lib.stream(device), threading.get_ident())
+    stream = _lib.stream(device)
+    who = (threading.get_ident(), _lib.capture(stream), stream)
     buf = kept.get(who)
     if buf is None:
-        while len(kept) >= SCRATCH_KEPT:                        # its memory goes back to its stream, behind what runs there
-            kept.pop(list(kept)[0], None)
-        buf = kept[who] = make()
+        for other in list(kept):                                # what is let go returns to its stream, behind what runs there
+            if len(kept) >= SCRATCH_KEPT or who[1] and other[1] not in (0, who[1]) and other[0] == who[0]:
+                kept.pop(other, None)
+        buf = kept[who] = MoEBuffers(size, _Shape(m), device, prefill=prefill, shared=m.shared, dtype=dtype)
     return buf
 
 

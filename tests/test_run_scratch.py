@@ -1,4 +1,4 @@
-"""``moe.run``'s scratch: one set a stream, a thread and a captured call (host logic without a GPU), and on the GPU calls on
+"""``moe.run``'s scratch: one set a stream, a thread and a capture (host logic without a GPU), and on the GPU calls on
 two streams and replays of two graphs beside one another with the bits of calls in a row."""
 
 import threading
@@ -39,15 +39,15 @@ def calls(monkeypatch):
 
     from tensorfold_b200 import _lib, moe
 
-    state = {"stream": 1, "capturing": False, "used": []}
+    state = {"stream": 1, "capture": 0, "used": []}
     monkeypatch.setattr(moe, "_scratch", {})
-    monkeypatch.setattr(moe, "_capturing", lambda device: state["capturing"], raising=False)
     monkeypatch.setattr(_lib, "stream", lambda device: state["stream"])
+    monkeypatch.setattr(_lib, "capture", lambda stream: state["capture"], raising=False)
     monkeypatch.setattr(moe, "layer", lambda x, m, buf, out: state["used"].append(buf))
     layer = routed("cpu")
 
-    def call(stream=1, capturing=False, rows=5, prefill=False):
-        state.update(stream=stream, capturing=capturing)
+    def call(stream=1, capture=0, rows=5, prefill=False):
+        state.update(stream=stream, capture=capture)
         moe.run(torch.zeros((rows, 128), dtype=BF), layer, prefill=prefill)
         return state["used"][-1]
 
@@ -69,10 +69,17 @@ def test_threads_do_not_share_scratch(calls):
     assert other[0] is not mine and calls() is mine
 
 
-def test_a_captured_call_has_scratch_of_its_own(calls):
-    eager = calls()
-    held = [calls(capturing=True), calls(capturing=True)]
-    assert held[0] is not held[1] and eager not in held and calls() is eager
+def test_a_capture_has_scratch_of_its_own(calls):
+    """Shared by the capture's calls on one stream, with no other capture and no eager call; the last capture's is let go
+    for the next one's."""
+
+    from tensorfold_b200 import moe
+
+    eager, first = calls(), calls(capture=7)
+    assert first is not eager and calls(capture=7) is first and calls(stream=2, capture=7) not in (first, eager)
+    second = calls(capture=8)
+    assert second not in (first, eager) and calls() is eager and calls(capture=8) is second
+    assert [sorted(who[1] for who in kept) for kept in moe._scratch.values()] == [[0, 8]]
 
 
 def test_scratch_is_bounded(calls):
@@ -104,6 +111,21 @@ def test_two_streams_run_layers_of_one_shape(kind):
     torch.cuda.synchronize()
     for k in (0, 1):
         assert all(torch.equal(y, want[k]) for y in got[k])
+
+
+@pytest.mark.gpu
+def test_captures_are_told_apart():
+    from tensorfold_b200 import _lib
+
+    s, dev, seen = torch.cuda.Stream(), torch.device("cuda", 0), []
+    torch.cuda.synchronize()
+    for _ in range(2):
+        with torch.cuda.graph(torch.cuda.CUDAGraph(), stream=s):
+            seen += [_lib.capture(_lib.stream(dev)), _lib.capture(_lib.stream(dev))]
+            torch.zeros((4,), device="cuda")
+    assert seen[0] == seen[1] != seen[2] == seen[3] and 0 not in seen
+    with torch.cuda.stream(s):
+        assert _lib.capture(_lib.stream(dev)) == 0
 
 
 @pytest.mark.gpu
