@@ -392,8 +392,10 @@ adapters_kernel(AdArgs g) {
     constexpr unsigned lanes = SH::SUM_ROWS * QUADS >= 32 ? 0xffffffffu : (1u << (SH::SUM_ROWS * QUADS % 32)) - 1;   // a row's fours are neighbours
 #pragma unroll
     for (int d = 1; d < QUADS; d *= 2) most = fmaxf(most, __shfl_xor_sync(lanes, most, d));
+    // the row's largest value into [1, 4), or near 1 as far as a power of two goes (fp32's largest and least values); a row with
+    // an infinity or NaN as it is
     int ex = 0;
-    if (most > 0.f && most <= 3.0e38f) ex = max(-100, min(100, ilogbf(most)));
+    if (most > 0.f && most <= 3.402823466e38f) ex = max(-126, min(126, ilogbf(most)));
     const float down = __uint_as_float((uint32_t)(127 - ex) << 23);        // 2^-ex: exact
 #pragma unroll
     for (int q = 0; q < 4; ++q) s[q] *= down;
