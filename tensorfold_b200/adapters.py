@@ -77,7 +77,7 @@ class Adapters:
         self.scale[i:i + 1].fill_(scale)
 
     def clear(self, i: int) -> None:
-        """Empty slot ``i``: its rows then come out as the base alone."""
+        """Empty slot ``i``: its rows then come out as the base alone, whatever their inputs hold."""
 
         i = self._slot(i)
         self.a[i].zero_()

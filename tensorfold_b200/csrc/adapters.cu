@@ -386,7 +386,7 @@ adapters_kernel(AdArgs g) {
     float most = 0.f;
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
-      s[q] *= scale;
+      s[q] = scale == 0.f ? 0.f : s[q] * scale;                            // an empty slot's row: whatever its inputs hold
       most = fmaxf(most, fabsf(s[q]));
     }
     constexpr unsigned lanes = SH::SUM_ROWS * QUADS >= 32 ? 0xffffffffu : (1u << (SH::SUM_ROWS * QUADS % 32)) - 1;   // a row's fours are neighbours

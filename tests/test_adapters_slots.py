@@ -54,3 +54,34 @@ def test_scales_at_the_ends_of_fp32(dtype, rank, rows):
         ad = adapters.make(a, b, 2.0 ** power)
         got = adapters.add(x, ad, plan, base)
         assert torch.equal(got.double(), delta * 2.0 ** power), power
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows", [6, 140])
+@pytest.mark.parametrize("rank", RANKS)
+@pytest.mark.parametrize("dtype", [BF, HF])
+def test_rows_of_empty_slots_are_the_base_whatever_their_inputs(dtype, rank, rows):
+    """A slot that was never filled and one that was emptied, under infinities, NaN and the type's largest value (a padded
+    batch): the base, rounded; the rows of a filled slot beside them as they are alone."""
+
+    from tensorfold_b200 import adapters
+
+    g = torch.Generator(device="cuda").manual_seed(7)
+
+    def normal(*shape):
+        return torch.randn(shape, generator=g, device="cuda")
+
+    ad = adapters.Adapters(3, rank, 72, 40, dtype, "cuda")
+    ad.put(0, normal(rank, 72) * 0.1, normal(40, rank))
+    ad.put(2, normal(rank, 72) * 0.1, normal(40, rank))
+    ad.clear(2)
+    ids = (torch.arange(rows, device="cuda") % 3).to(torch.int32)
+    plan = adapters.Plan(rows, 3, "cuda")
+    adapters.route(ids, plan)
+    x, base = normal(rows, 72).to(dtype), normal(rows, 40)
+    clean = adapters.add(x, ad, plan, base, dtype=dtype)
+    empty = (ids != 0).nonzero()[:, 0]
+    for i, value in enumerate((float("inf"), float("-inf"), float("nan"), torch.finfo(dtype).max)):
+        x[empty[i::4], i::7] = value
+    got = adapters.add(x, ad, plan, base, dtype=dtype)
+    assert torch.equal(got[empty], base[empty].to(dtype)) and torch.equal(got[ids == 0], clean[ids == 0])
