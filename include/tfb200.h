@@ -358,9 +358,10 @@ int tfb_experts16_block(int fp16, const void* x, int64_t x_stride, int rows, con
 
 /* out[m] = base[m] + scale[i] * B[i] (A[i] x[m]) with i = ids[m], the base alone where i is outside 0..count-1.  x
  * [rows, k], a [count, rank, k], b [count, n, rank] in bf16 or fp16 (fp16 != 0); k and rank multiples of 8, rank at most
- * 128, zeros behind an adapter's own rank; scale 0 with zeros in b: the base alone, whatever x holds.  base and out: fp32 (0), bf16 (1) or fp16 (2) rows *_stride elements apart; out
- * may be base.  items, counts, members, max_items: tfb_plan's tables of the ids with items of at most 64 rows, or nulls:
- * every row on its own (for few rows).  A row's bits depend on its own row alone. */
+ * 128, zeros behind an adapter's own rank.  Where scale is 0 and b holds zeros (an empty slot) the base alone, whatever x
+ * holds.  base and out: fp32 (0), bf16 (1) or fp16 (2) rows *_stride elements apart; out may be base.  items, counts,
+ * members, max_items: tfb_plan's tables of the ids with items of at most 64 rows, or nulls: every row on its own (for few
+ * rows).  A row's bits depend on its own row alone. */
 int tfb_adapters(int fp16, const void* x, int64_t x_stride, const void* a, const void* b, const float* scale, int rank,
                  int k, int n, const int32_t* ids, int rows, int count, const int32_t* items, const int32_t* counts,
                  const int32_t* members, int64_t max_items, const void* base, int base_type, int64_t base_stride,

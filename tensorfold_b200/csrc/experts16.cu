@@ -11,8 +11,9 @@
 // What bounds it.  Few pairs an expert: HBM - 64 tokens of 128 experts (2048 x 768, top 8), gate/up 119 us for 793 MB, 1.02 of
 // the copy rate; one token 14 us for 50 MB, of which 9 stream and the rest is start, plan and end.  Some hundred pairs: HBM
 // and the tensor pipe in turn - 1999 tokens 145 us, DRAM 73 % of its peak, tensor pipe 40 % busy.  Many: the tensor pipe, 79 %
-// busy at 4096 tokens of 32 experts (160 us, 1290 TFLOP/s), and on long runs the power cap: 8192 tokens of 160 experts
-// (4096 x 1536) run at 877 MHz and 873 TFLOP/s, 0.82 of what the pipe can do at that clock.
+// busy at 4096 tokens of 32 experts (160 us, 1290 TFLOP/s), and on long runs the clock that the power cap leaves it: 8192 tokens
+// of 160 experts (4096 x 1536) run at 877 MHz and 873 TFLOP/s, 0.82 of what the pipe can do at that clock (a plain 8192-cubed
+// library product holds 1327 MHz and 1380 TFLOP/s under the same cap, so an operation costs more energy here).
 
 #include "api.h"
 #include "common.cuh"

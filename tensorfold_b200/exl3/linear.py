@@ -35,7 +35,8 @@ def _stream(t: torch.Tensor) -> int:
 
 @dataclass
 class Exl3Linear:
-    """One EXL3 layer on the GPU: trellis int16 [K/16, N/16, 16 * bits] in place, fp16 scales, optional fp16 bias."""
+    """One EXL3 layer on the GPU: trellis int16 [K/16, N/16, 16 * bits] in place, fp16 scales, optional fp16 bias.  A call counts
+    its split sums in the layer's own counters, so calls of one layer follow one another (on one stream, or ordered)."""
 
     trellis: torch.Tensor
     suh: torch.Tensor             # fp16 [K]
